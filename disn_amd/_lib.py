@@ -27,6 +27,33 @@ class DisnMcGrid(ctypes.Structure):
                 ("own0", ctypes.c_int32), ("own1", ctypes.c_int32)]
 
 
+class DisnLinear(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32), ("act", ctypes.c_int32), ("w_nk", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("m", c_int64), ("n", c_int64), ("k", c_int64), ("x", c_void_p), ("ldx", c_int64), ("w", c_void_p),
+                ("ldw", c_int64), ("bias", c_void_p), ("residual", c_void_p), ("ldr", c_int64), ("y", c_void_p),
+                ("ldy", c_int64), ("pre", c_void_p), ("ldp", c_int64)]
+
+
+class DisnLinearGrad(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32), ("act", ctypes.c_int32), ("w_nk", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("m", c_int64), ("n", c_int64), ("k", c_int64), ("dy", c_void_p), ("lddy", c_int64), ("x", c_void_p),
+                ("ldx", c_int64), ("w", c_void_p), ("ldw", c_int64), ("pre", c_void_p), ("ldp", c_int64), ("dx", c_void_p),
+                ("lddx", c_int64), ("dw", c_void_p), ("lddw", c_int64), ("db", c_void_p)]
+
+
+class DisnLayerNorm(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32), ("reserved", ctypes.c_int32), ("rows", c_int64), ("d", c_int64), ("x", c_void_p),
+                ("ldx", c_int64), ("weight", c_void_p), ("bias", c_void_p), ("eps", ctypes.c_double), ("y", c_void_p),
+                ("ldy", c_int64), ("mean", c_void_p), ("rstd", c_void_p)]
+
+
+class DisnLayerNormGrad(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32), ("reserved", ctypes.c_int32), ("rows", c_int64), ("d", c_int64), ("dy", c_void_p),
+                ("lddy", c_int64), ("x", c_void_p), ("ldx", c_int64), ("mean", c_void_p), ("rstd", c_void_p),
+                ("weight", c_void_p), ("residual", c_void_p), ("ldr", c_int64), ("dx", c_void_p), ("lddx", c_int64),
+                ("dweight", c_void_p), ("dbias", c_void_p)]
+
+
 # name -> (restype, argtypes); mirrors include/disn.h one to one
 SIGNATURES = {
     "disn_create": (c_int, [c_int, ctypes.POINTER(c_void_p)]),
@@ -46,6 +73,13 @@ SIGNATURES = {
     "disn_sample_features": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "disn_vgg_set_weights": (c_int, [c_void_p, c_int, ctypes.POINTER(DisnVggWeights)]),
     "disn_vgg_forward": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, ctypes.POINTER(c_void_p), c_void_p, c_void_p]),
+    "disn_linear_workspace": (c_int, [c_void_p, ctypes.POINTER(DisnLinear), ctypes.POINTER(ctypes.c_size_t)]),
+    "disn_linear": (c_int, [c_void_p, ctypes.POINTER(DisnLinear), c_void_p, ctypes.c_size_t, c_void_p]),
+    "disn_linear_backward_workspace": (c_int, [c_void_p, ctypes.POINTER(DisnLinearGrad), ctypes.POINTER(ctypes.c_size_t)]),
+    "disn_linear_backward": (c_int, [c_void_p, ctypes.POINTER(DisnLinearGrad), c_void_p, ctypes.c_size_t, c_void_p]),
+    "disn_layer_norm": (c_int, [c_void_p, ctypes.POINTER(DisnLayerNorm), c_void_p]),
+    "disn_layer_norm_backward_workspace": (c_int, [c_void_p, ctypes.POINTER(DisnLayerNormGrad), ctypes.POINTER(ctypes.c_size_t)]),
+    "disn_layer_norm_backward": (c_int, [c_void_p, ctypes.POINTER(DisnLayerNormGrad), c_void_p, ctypes.c_size_t, c_void_p]),
     "disn_mc_count": (c_int, [c_void_p, c_void_p, ctypes.POINTER(DisnMcGrid), c_float,
                               ctypes.POINTER(c_uint64), c_void_p]),
     "disn_mc_emit": (c_int, [c_void_p, c_void_p, c_uint64, c_uint64, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),

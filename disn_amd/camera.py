@@ -50,14 +50,18 @@ def rotation_from_ortho6d(p):
     return torch.stack((x, y, z), dim=2)
 
 
-def pred_trans_mat(embedding, weights):
-    """embedding: [B,1024] tensor (any device) -> pred_trans_mat [B,4,3]."""
+def pred_trans_mat(embedding, weights, ctx=None):
+    """embedding: [B,1024] tensor (any device) -> pred_trans_mat [B,4,3].  With a Context the heads' layers run through
+    its dense layer (the embedding on its device); otherwise through torch."""
     e = embedding.reshape(-1, 1024).float()
     w = {k: torch.as_tensor(v, dtype=torch.float32, device=e.device) for k, v in weights.items()}
 
     def head(name):
         h = e
         for li in (1, 2, 3):
+            if ctx is not None:
+                h = ctx.linear(h, w["%s/fc%d/weights" % (name, li)], w["%s/fc%d/biases" % (name, li)], act="relu" if li < 3 else "none")
+                continue
             h = h @ w["%s/fc%d/weights" % (name, li)] + w["%s/fc%d/biases" % (name, li)]
             if li < 3:
                 h = torch.relu(h)

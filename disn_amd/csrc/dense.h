@@ -1,0 +1,84 @@
+// dense.h -- what linear.hip and norm.hip share: element types, unaligned vector loads and stores, the sum over
+// partial column sums.
+#pragma once
+#include "common.h"
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+// 16 bytes of T.  Rows start at any address that fits T (odd widths, slices), so the accesses go through memcpy with
+// T's own alignment: hipcc makes one global_load/store_dwordx4 of each, which the hardware takes at any address.
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  T v[N];
+};
+
+template <typename T>
+__device__ __forceinline__ Vec<T> load_vec(const T* p) {
+  Vec<T> r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
+// the first n (<= N) values at p, zeros behind them; nothing beyond p[n - 1] is read
+template <typename T>
+__device__ __forceinline__ Vec<T> load_vec(const T* p, int n) {
+  if (n >= Vec<T>::N) return load_vec(p);
+  Vec<T> r;
+#pragma unroll
+  for (int i = 0; i < Vec<T>::N; ++i) r.v[i] = i < n ? p[i] : (T)0.0f;
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T>& r, int n) {
+  if (n >= Vec<T>::N) {
+    __builtin_memcpy(p, &r, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i)
+      if (i < n) p[i] = r.v[i];
+  }
+}
+
+// Sum of partial column sums: out[c] = part[0][c] + part[1][c] + ... .  A workgroup takes 16 columns; its 16 groups of
+// 16 threads add every 16th partial each, and the group sums are added in order (a fixed association).
+// Columns [0, d) go to out0, [d, 2 d) to out1 (a layer norm's two gradients; ncols = d or 2 d), either may be null.
+template <typename T>
+__global__ __launch_bounds__(256) void k_sum_partials(const float* __restrict__ part, int nparts, int64_t ncols, int64_t d,
+                                                      T* __restrict__ out0, T* __restrict__ out1) {
+  __shared__ float lds[16][17];
+  const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
+  const int64_t col = (int64_t)blockIdx.x * 16 + c;
+  float s = 0.0f;
+  if (col < ncols) {
+#pragma unroll 4
+    for (int p = g; p < nparts; p += 16) s += part[(size_t)p * ncols + col];
+  }
+  lds[g][c] = s;
+  __syncthreads();
+  if (g == 0 && col < ncols) {
+    float t = lds[0][c];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) t += lds[i][c];
+    T* out = col < d ? out0 : out1;
+    if (out) out[col < d ? col : col - d] = (T)t;
+  }
+}
+
+inline bool dense_type_ok(int t) { return t == DISN_F32 || t == DISN_BF16 || t == DISN_F16; }
+inline size_t dense_type_size(int t) { return t == DISN_F32 ? 4 : 2; }
+inline bool dense_aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+inline bool dense_size_ok(int64_t v) { return v >= 0 && v <= 1 << 30; }
+// a matrix argument: present, fits its type's alignment, row distance possible.  Row distances are bounded so that
+// rows * ld * size stays inside 63 bits.
+inline bool dense_matrix_ok(const void* p, int64_t rows, int64_t cols, int64_t ld, size_t size, bool input) {
+  if (rows == 0 || cols == 0) return true;
+  return p && dense_aligned(p, size) && ld <= (int64_t)1 << 31 && (ld >= cols || (input && ld == 0) || (rows == 1 && ld >= 0));
+}
+
+template <typename F>
+inline int dense_dispatch(int type, F&& f) {
+  if (type == DISN_F32) return f((float)0);
+  if (type == DISN_BF16) return f((bf16_t)0.0f);
+  return f((f16_t)0.0f);
+}

@@ -1,0 +1,1007 @@
+// linear.hip -- the dense layer y = act(x W + b) + r and its gradients (include/disn.h).
+//
+// Forward and both gradients are one product C(i, j) = sum over r of A(i, r) B(j, r) with different operands:
+//   y   i = row, j = output, r = input     A = x                    B = W
+//   dx  i = row, j = input,  r = output    A = dz                   B = W
+//   dW  r = row                            A = x, B = dz ([k][n]) or A = dz, B = x ([n][k])
+// An operand lies "along" r (its r values are contiguous) or "across" (its i values are, rows of r).
+//
+// Three kernels compute it, chosen by size (plan() below):
+//   k_tile   large products: 128- or 256-wide tiles through LDS on the matrix cores
+//   k_small  products of a few tens of microseconds and less: no LDS tiles, the waves of a workgroup share the sum
+//   k_rows_* at most 16 rows times a large matrix: W streams past at memory speed
+#include "dense.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(16))) float floatx16;
+typedef __attribute__((ext_vector_type(4))) float floatx4;
+typedef __attribute__((ext_vector_type(4))) short shortx4;
+typedef __attribute__((ext_vector_type(8))) short shortx8;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((address_space(3))) shortx4 lds_shortx4;
+
+// ---- activations ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float activate(float z, int act) {
+  switch (act) {
+    case DISN_ACT_RELU: return z < 0.0f ? 0.0f : z;   // NaN stays
+    case DISN_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case DISN_ACT_SILU: return z / (1.0f + expf(-z));
+    default: return z;
+  }
+}
+// act'(z)
+__device__ __forceinline__ float slope(float z, int act) {
+  switch (act) {
+    case DISN_ACT_RELU: return z > 0.0f ? 1.0f : z <= 0.0f ? 0.0f : z;
+    case DISN_ACT_GELU:
+      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * (0.39894228040143268f * expf(-0.5f * z * z));
+    case DISN_ACT_SILU: {
+      const float s = 1.0f / (1.0f + expf(-z));
+      return s * (1.0f + z * (1.0f - s));
+    }
+    default: return 1.0f;
+  }
+}
+
+// ---- what becomes of a finished sum ------------------------------------------------------------------------------
+struct Epilogue {
+  const void *bias, *residual;
+  void *pre, *out;
+  int64_t ldr, ldp, ldo;
+  int act;
+};
+template <typename T>
+__device__ __forceinline__ void finish_one(const Epilogue& e, int64_t row, int col, float z) {
+  if (e.bias) z += (float)((const T*)e.bias)[col];
+  if (e.pre) ((T*)e.pre)[row * e.ldp + col] = (T)z;
+  float y = activate(z, e.act);
+  if (e.residual) y += (float)((const T*)e.residual)[row * e.ldr + col];
+  ((T*)e.out)[row * e.ldo + col] = (T)y;
+}
+// n (>= 1) of Vec<T>::N values in a row
+template <typename T>
+__device__ __forceinline__ void finish_vec(const Epilogue& e, int64_t row, int col, float (&z)[Vec<T>::N], int n) {
+  constexpr int N = Vec<T>::N;
+  if (e.bias) {
+    const Vec<T> b = load_vec((const T*)e.bias + col, n);
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] += (float)b.v[i];
+  }
+  Vec<T> o;
+  if (e.pre) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) o.v[i] = (T)z[i];
+    store_vec((T*)e.pre + row * e.ldp + col, o, n);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) z[i] = activate(z[i], e.act);
+  if (e.residual) {
+    const Vec<T> r = load_vec((const T*)e.residual + row * e.ldr + col, n);
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] += (float)r.v[i];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) o.v[i] = (T)z[i];
+  store_vec((T*)e.out + row * e.ldo + col, o, n);
+}
+
+// sums the partial products of a split r (0 of them: an empty sum) in order and finishes them
+template <typename T>
+__global__ __launch_bounds__(256) void k_finish(const float* __restrict__ part, int nparts, int64_t M, int N, Epilogue e) {
+  constexpr int V = Vec<T>::N;
+  const int64_t per_row = (N + V - 1) / V, total = M * per_row;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+    const int64_t row = t / per_row;
+    const int col = (int)(t - row * per_row) * V, n = N - col;
+    float z[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) z[i] = 0.0f;
+#pragma unroll 2
+    for (int p = 0; p < nparts; ++p) {
+      const float* s = part + ((size_t)p * M + row) * N + col;
+#pragma unroll
+      for (int i = 0; i < V; i += 4) {
+        const Vec<float> v = load_vec(s + (i < n ? i : 0), i < n ? n - i : 0);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) z[i + q] += v.v[q];
+      }
+    }
+    finish_vec<T>(e, row, col, z, n);
+  }
+}
+
+// ---- k_tile --------------------------------------------------------------------------------------------------------
+// A workgroup computes a BM x BN tile of C, r in stages of KT.  The stage after the next is on its way from memory to
+// registers while the next lies in one LDS buffer and the waves multiply the present one from the other: one barrier a
+// stage.  Waves are WM x WN; each has MB x NB tiles of v_mfma_f32_32x32x16.
+//
+// 16-bit types go to the matrix cores as they are.  fp32 is cut into three bf16 terms x = h + m + l (each the rounded
+// rest of the one before; 8 + 8 + 8 bits hold fp32's 24, so the sum is exact) and the six products
+// hh, hm, mh, mm, hl, lh are accumulated in fp32; what is left out (ml, lm, ll) is below 2^-24 of a product, as an
+// FMA's rounding is.  Six bf16 MFMAs take 6/16 of the time of one fp32 MFMA of the same size.  Infinities,
+// NaN and intermediate overflow cannot be cut; a tile whose sums are not all finite is computed again by plain FMAs.
+//
+// LDS: an operand along r as [16 r][i][32 bytes] (a wave's fragment is 1 KB in one piece; 32 bytes between the 16-r
+// blocks put the eight lanes that store one row on different banks); an operand across r as [r][i] with 64 bytes
+// between rows, read through ds_read_b64_tr_b16, which hands each lane 4 r values of its i.
+template <typename T>
+struct Mma {
+  static constexpr int planes = 1;
+  static constexpr int KT = 64;
+};
+template <>
+struct Mma<float> {
+  static constexpr int planes = 3;
+  static constexpr int KT = 16;
+};
+
+template <typename T>
+__device__ __forceinline__ floatx16 mfma(shortx8 a, shortx8 b, floatx16 c) {
+  if constexpr (__is_same(T, f16_t))
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <typename T, bool ACROSS, int ROWS, int THREADS>
+struct Operand {
+  static constexpr int KT = Mma<T>::KT, P = Mma<T>::planes, V = Vec<T>::N;
+  static constexpr int PER_LINE = (ACROSS ? ROWS : KT) / V;    // 16-byte pieces in a contiguous run
+  static constexpr int Q = ROWS * KT / V / THREADS;            // pieces a thread moves per stage
+  static constexpr int LINE = ROWS * 2 + 64;                   // bytes of one r (across)
+  static constexpr int BLOCK = ROWS * 32 + 32;                 // bytes of 16 r (along)
+  static constexpr int PLANE = ACROSS ? KT * LINE : KT / 16 * BLOCK;
+  static constexpr int BYTES = PLANE * P;
+  static_assert(Q * THREADS * V == ROWS * KT, "pieces");
+
+  const T* ptr[Q];
+  int64_t ld;
+  int left;          // i values in the tile
+  Vec<T> reg[Q];
+
+  __device__ __forceinline__ void init(const T* p, int64_t ld_, int i0, int n_i, int64_t k0) {
+    ld = ld_;
+    left = n_i - i0;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int t = threadIdx.x + q * THREADS, line = t / PER_LINE, c = t % PER_LINE * V;
+      // places outside the matrix read its nearest line or first piece instead: they only reach sums nobody stores
+      if (ACROSS)
+        ptr[q] = p + (k0 + line) * ld + i0 + (c < left ? c : 0);
+      else
+        ptr[q] = p + (int64_t)(i0 + (line < left ? line : left - 1)) * ld + k0 + c;
+    }
+  }
+  // the next stage, of which `have` (>= 1) r values exist; zeros behind them
+  __device__ __forceinline__ void fetch(int have) {
+    if (have >= KT && (!ACROSS || left >= ROWS)) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) reg[q] = load_vec(ptr[q]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int t = threadIdx.x + q * THREADS, line = t / PER_LINE, c = t % PER_LINE * V;
+        if (ACROSS) {
+          const int n = c < left ? left - c : left;
+          reg[q] = load_vec(ptr[q] - (line < have ? 0 : line * ld), line < have ? n : 0);
+        } else {
+          reg[q] = load_vec(ptr[q] - (c < have ? 0 : c), have - c);
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) ptr[q] += ACROSS ? KT * ld : KT;
+  }
+  __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int t = threadIdx.x + q * THREADS, line = t / PER_LINE, c = t % PER_LINE * V;
+      char* dst = lds + (ACROSS ? line * LINE + c * 2 : (c >> 4) * BLOCK + line * 32 + (c & 15) * 2);
+      if constexpr (P == 1) {
+        __builtin_memcpy(__builtin_assume_aligned(dst, 16), &reg[q], 16);
+      } else {
+        float rest[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rest[i] = reg[q].v[i];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          bf16_t term[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            term[i] = (bf16_t)rest[i];
+            rest[i] -= (float)term[i];
+          }
+          __builtin_memcpy(__builtin_assume_aligned(dst + p * PLANE, 8), term, 8);
+        }
+      }
+    }
+  }
+  // fragment of 32 i values from i, 16 r values from 16 s: lane (l & 31) holds i + (l & 31), r = 8 (l >> 5) + 0..7
+  static __device__ __forceinline__ shortx8 fragment(const char* lds, int plane, int i, int s) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (ACROSS) {
+      // a group of 16 lanes reads 4 r x 16 i: lane q supplies r = q >> 2, i = 4 (q & 3), and gets i = q of all four
+      const int q = lane & 15;
+      const char* p = lds + plane * PLANE + (16 * s + 8 * (lane >> 5) + (q >> 2)) * LINE + (i + (lane & 16) + 4 * (q & 3)) * 2;
+      const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)(p));
+      const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)(p + 4 * LINE));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      const char* p = lds + plane * PLANE + s * BLOCK + (i + (lane & 31)) * 32 + (lane >> 5) * 16;
+      return *(const shortx8*)p;
+    }
+  }
+};
+
+struct TileArgs {
+  const void *A, *B;
+  int64_t lda, ldb;
+  int M, N;
+  int64_t K, per;          // r values in all and per split (a multiple of KT)
+  int mt, nt, splits;
+  float* part;             // [splits][M][N], splits > 1
+  Epilogue e;
+};
+
+template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64) void k_tile(TileArgs a) {
+  constexpr int THREADS = WM * WN * 64, MB = BM / WM / 32, NB = BN / WN / 32, KT = Mma<T>::KT, P = Mma<T>::planes;
+  typedef Operand<T, A_ACROSS, BM, THREADS> OpA;
+  typedef Operand<T, B_ACROSS, BN, THREADS> OpB;
+  constexpr int BUF = OpA::BYTES + OpB::BYTES;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  // Workgroups go to the 8 XCDs in turn; consecutive tiles share operands, so each XCD (own L2) takes a run of them.
+  const int total = a.mt * a.nt * a.splits, run = total >> 3, rest = total & 7, xcd = blockIdx.x & 7;
+  int id = (blockIdx.x >> 3) + xcd * run + (xcd < rest ? xcd : rest);
+  const int tn = id % a.nt;
+  id /= a.nt;
+  const int tm = id % a.mt, split = id / a.mt;
+  const int i0 = tm * BM, j0 = tn * BN;
+  const int64_t k0 = split * a.per;
+  const int have = (int)(a.K - k0 < a.per ? a.K - k0 : a.per), stages = (have + KT - 1) / KT;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wi = wave / WN * (MB * 32), wj = wave % WN * (NB * 32);
+
+  floatx16 acc[MB][NB];
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int g = 0; g < 16; ++g) acc[m][n][g] = 0.0f;
+
+  OpA A;
+  OpB B;
+  A.init((const T*)a.A, a.lda, i0, a.M, k0);
+  B.init((const T*)a.B, a.ldb, j0, a.N, k0);
+  A.fetch(have);
+  B.fetch(have);
+  A.store(lds);
+  B.store(lds + OpA::BYTES);
+  if (stages > 1) {
+    A.fetch(have - KT);
+    B.fetch(have - KT);
+  }
+  for (int s = 0; s < stages; ++s) {
+    __syncthreads();   // stage s is in LDS for everyone, stage s - 1 has been read by everyone
+    const char* cur = lds + (s & 1) * BUF;
+    char* nxt = lds + (~s & 1) * BUF;
+    if (s + 1 < stages) {
+      A.store(nxt);
+      B.store(nxt + OpA::BYTES);
+    }
+    if (s + 2 < stages) {
+      A.fetch(have - (s + 2) * KT);
+      B.fetch(have - (s + 2) * KT);
+    }
+#pragma unroll
+    for (int q = 0; q < KT / 16; ++q) {
+      shortx8 b[NB][P];
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int p = 0; p < P; ++p) b[n][p] = OpB::fragment(cur + OpA::BYTES, p, wj + n * 32, q);
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        shortx8 f[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) f[p] = OpA::fragment(cur, p, wi + m * 32, q);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          if constexpr (P == 3) {
+            acc[m][n] = mfma<T>(f[2], b[n][0], acc[m][n]);
+            acc[m][n] = mfma<T>(f[0], b[n][2], acc[m][n]);
+            acc[m][n] = mfma<T>(f[1], b[n][1], acc[m][n]);
+            acc[m][n] = mfma<T>(f[1], b[n][0], acc[m][n]);
+            acc[m][n] = mfma<T>(f[0], b[n][1], acc[m][n]);
+          }
+          acc[m][n] = mfma<T>(f[0], b[n][0], acc[m][n]);
+        }
+      }
+    }
+  }
+
+  // lane's place in a 32 x 32 tile of C: j = l & 31, i = (g & 3) + 8 (g >> 2) + 4 (l >> 5)
+  const int cj = lane & 31, ci = 4 * (lane >> 5);
+  if constexpr (P == 3) {
+    bool bad = false;
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int g = 0; g < 16; ++g) bad |= !(fabsf(acc[m][n][g]) <= 3.4028235e38f);
+    if (__syncthreads_or(bad)) {
+      const int64_t ai = A_ACROSS ? 1 : a.lda, ar = A_ACROSS ? a.lda : 1, bj = B_ACROSS ? 1 : a.ldb, br = B_ACROSS ? a.ldb : 1;
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const int j = min(j0 + wj + n * 32 + cj, a.N - 1);
+          const float* pb = (const float*)a.B + j * bj + k0 * br;
+          const float* pa = (const float*)a.A + k0 * ar;
+          int64_t row[16];
+#pragma unroll
+          for (int g = 0; g < 16; ++g) row[g] = min(i0 + wi + m * 32 + ci + (g & 3) + 8 * (g >> 2), a.M - 1) * ai;
+          floatx16 c;
+#pragma unroll
+          for (int g = 0; g < 16; ++g) c[g] = 0.0f;
+          for (int k = 0; k < have; ++k) {
+            const float bv = pb[k * br];
+#pragma unroll
+            for (int g = 0; g < 16; ++g) c[g] = fmaf(pa[row[g] + k * ar], bv, c[g]);
+          }
+          acc[m][n] = c;
+        }
+    }
+  }
+
+  if (a.splits > 1) {
+    float* part = a.part + (size_t)split * a.M * a.N;
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int g = 0; g < 16; ++g) {
+          const int i = i0 + wi + m * 32 + ci + (g & 3) + 8 * (g >> 2), j = j0 + wj + n * 32 + cj;
+          if (i < a.M && j < a.N) part[(size_t)i * a.N + j] = acc[m][n][g];
+        }
+    return;
+  }
+  // each wave turns its 32 rows at a time through LDS, so that a lane finishes 16 bytes of one row
+  constexpr int W = NB * 32, V = Vec<T>::N, STRIDE = W + 4;
+  static_assert(32 * STRIDE * 4 * WM * WN <= 2 * BUF, "the turned tiles fit into the stage buffers");
+  __syncthreads();
+  float* mine = (float*)lds + wave * (32 * STRIDE);
+#pragma unroll
+  for (int m = 0; m < MB; ++m) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int g = 0; g < 16; ++g) mine[(ci + (g & 3) + 8 * (g >> 2)) * STRIDE + n * 32 + cj] = acc[m][n][g];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int q = 0; q < 32 * W / V / 64; ++q) {
+      const int t = lane + q * 64, r = t / (W / V), c = t % (W / V) * V;
+      const int i = i0 + wi + m * 32 + r, j = j0 + wj + c;
+      if (i >= a.M || j >= a.N) continue;
+      float z[V];
+      __builtin_memcpy(z, __builtin_assume_aligned(mine + r * STRIDE + c, 16), sizeof z);
+      finish_vec<T>(a.e, i, j, z, a.N - j);
+    }
+  }
+}
+
+// ---- k_small -------------------------------------------------------------------------------------------------------
+// Small products are bound by latency, not by the matrix cores: operands go straight from memory (or L2) into fragments
+// of v_mfma_f32_16x16x4, 16-bit types widened (exact), 16 r values a step.  Eight waves a workgroup: long sums
+// (KS = 8) give every wave an eighth of the steps of one 16 x 16 tile and add the eight in order; short ones (KS = 1) give
+// every wave a tile of its own.  An operand can be gated, dz = dy act'(pre), as it is read, and its sum over r
+// (the bias's gradient) taken along: a backward pass of this size is one launch.
+struct SmallOperand {
+  const void* p;
+  const void* gate;   // z, or null
+  int64_t ld, ldg;
+};
+struct SmallArgs {
+  SmallOperand A, B;
+  int M, N, K, mt, nt, ks, act;
+  void* rsum;         // sum over r of operand B (rsum_of_a: of A), or null
+  int rsum_of_a;
+  Epilogue e;
+};
+constexpr int SMALL_WAVES = 8;
+
+// r = r0 .. r0 + 3 (those below K) of line i (clamped to the matrix by the caller)
+template <typename T, bool ACROSS, bool FULL>
+__device__ __forceinline__ floatx4 small_load(const void* p_, int64_t ld, int i, int r0, int K) {
+  const T* p = (const T*)p_;
+  floatx4 v;
+  if constexpr (!ACROSS && FULL) {
+    T t[4];
+    __builtin_memcpy(t, p + i * ld + r0, sizeof t);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (float)t[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool in = FULL || r0 + e < K;
+      const int r = in ? r0 + e : 0;
+      const float x = (float)p[ACROSS ? r * ld + i : i * ld + r];
+      v[e] = in ? x : 0.0f;
+    }
+  }
+  return v;
+}
+template <typename T, bool ACROSS, bool GATED, bool FULL>
+__device__ __forceinline__ floatx4 small_operand(const SmallOperand& o, int i, int r0, int K, int act) {
+  floatx4 v = small_load<T, ACROSS, FULL>(o.p, o.ld, i, r0, K);
+  if constexpr (GATED) {
+    if (act != DISN_ACT_NONE) {
+      const floatx4 z = small_load<T, ACROSS, FULL>(o.gate, o.ldg, i, r0, K);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] *= FULL || r0 + e < K ? slope(z[e], act) : 1.0f;
+    }
+  }
+  return v;
+}
+
+template <typename T, bool A_ACROSS, bool B_ACROSS, bool A_GATED, bool B_GATED, int KS>
+__device__ __forceinline__ void small_product(const SmallArgs& a, int block, float (*lds)[256], float (*lds_sum)[16]) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), idx = lane & 15, quad = lane >> 4;
+  constexpr int JW = SMALL_WAVES / KS;   // tiles along j of a workgroup
+  const int nt = (a.nt + JW - 1) / JW, ti = block / nt, tj = (block - ti * nt) * JW + (KS == 1 ? wave : 0);
+  const int i0 = ti * 16, j0 = tj * 16;
+  if (KS == 1 && tj >= a.nt) return;
+  const int i = min(i0 + idx, a.M - 1), j = min(j0 + idx, a.N - 1);
+  const int full = a.K >> 4;
+  floatx4 acc = {0, 0, 0, 0};
+  float sum = 0.0f;
+  auto step = [&](floatx4 av, floatx4 bv) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(av[e], bv[e], acc, 0, 0, 0);
+    if constexpr (A_GATED || B_GATED) {
+      const floatx4 g = a.rsum_of_a ? av : bv;
+      sum += (g[0] + g[1]) + (g[2] + g[3]);
+    }
+  };
+  int c = KS == 1 ? 0 : wave;
+  for (; c + 3 * KS < full; c += 4 * KS) {
+    floatx4 av[4], bv[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      av[u] = small_operand<T, A_ACROSS, A_GATED, true>(a.A, i, (c + u * KS) * 16 + quad * 4, a.K, a.act);
+      bv[u] = small_operand<T, B_ACROSS, B_GATED, true>(a.B, j, (c + u * KS) * 16 + quad * 4, a.K, a.act);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) step(av[u], bv[u]);
+  }
+  for (; c < full; c += KS)
+    step(small_operand<T, A_ACROSS, A_GATED, true>(a.A, i, c * 16 + quad * 4, a.K, a.act),
+         small_operand<T, B_ACROSS, B_GATED, true>(a.B, j, c * 16 + quad * 4, a.K, a.act));
+  if ((a.K & 15) && c == full)
+    step(small_operand<T, A_ACROSS, A_GATED, false>(a.A, i, c * 16 + quad * 4, a.K, a.act),
+         small_operand<T, B_ACROSS, B_GATED, false>(a.B, j, c * 16 + quad * 4, a.K, a.act));
+  const bool want_sum = (A_GATED || B_GATED) && a.rsum && (a.rsum_of_a ? tj == 0 : ti == 0);
+  if (A_GATED || B_GATED) {
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+  }
+  // lane's place in the tile: j = l & 15, i = 4 (l >> 4) + g
+  if constexpr (KS == 1) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      if (i0 + quad * 4 + g < a.M && j0 + idx < a.N) finish_one<T>(a.e, i0 + quad * 4 + g, j0 + idx, acc[g]);
+    const int at = (a.rsum_of_a ? i0 : j0) + idx;
+    if (want_sum && quad == 0 && at < (a.rsum_of_a ? a.M : a.N)) ((T*)a.rsum)[at] = (T)sum;
+  } else {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) lds[wave][(quad * 4 + g) * 16 + idx] = acc[g];
+    if (quad == 0) lds_sum[wave][idx] = sum;
+    __syncthreads();
+    const int t = threadIdx.x;
+    if (t < 256) {
+      float z = lds[0][t];
+#pragma unroll
+      for (int w = 1; w < KS; ++w) z += lds[w][t];
+      if (i0 + (t >> 4) < a.M && j0 + (t & 15) < a.N) finish_one<T>(a.e, i0 + (t >> 4), j0 + (t & 15), z);
+    } else if (want_sum && t < 272) {
+      float z = lds_sum[0][t & 15];
+#pragma unroll
+      for (int w = 1; w < KS; ++w) z += lds_sum[w][t & 15];
+      const int at = (a.rsum_of_a ? i0 : j0) + (t & 15);
+      if (at < (a.rsum_of_a ? a.M : a.N)) ((T*)a.rsum)[at] = (T)z;
+    }
+  }
+}
+
+template <typename T, bool B_ACROSS>
+__global__ __launch_bounds__(SMALL_WAVES * 64) void k_small(SmallArgs a) {
+  __shared__ float lds[SMALL_WAVES][256];
+  __shared__ float lds_sum[SMALL_WAVES][16];
+  if (a.ks == 1) small_product<T, false, B_ACROSS, false, false, 1>(a, blockIdx.x, lds, lds_sum);
+  else small_product<T, false, B_ACROSS, false, false, SMALL_WAVES>(a, blockIdx.x, lds, lds_sum);
+}
+// dx and dW (with the bias's gradient) of one layer in one launch: the first `split` workgroups compute dx
+template <typename T, bool W_NK>
+__global__ __launch_bounds__(SMALL_WAVES * 64) void k_small_backward(SmallArgs dx, SmallArgs dw, int split) {
+  __shared__ float lds[SMALL_WAVES][256];
+  __shared__ float lds_sum[SMALL_WAVES][16];
+  if ((int)blockIdx.x < split) {
+    if (dx.ks == 1) small_product<T, false, W_NK, true, false, 1>(dx, blockIdx.x, lds, lds_sum);
+    else small_product<T, false, W_NK, true, false, SMALL_WAVES>(dx, blockIdx.x, lds, lds_sum);
+  } else {
+    if (dw.ks == 1) small_product<T, true, true, W_NK, !W_NK, 1>(dw, blockIdx.x - split, lds, lds_sum);
+    else small_product<T, true, true, W_NK, !W_NK, SMALL_WAVES>(dw, blockIdx.x - split, lds, lds_sum);
+  }
+}
+
+// ---- k_rows: few rows times a large matrix ---------------------------------------------------------------------------
+// W is read once at memory speed, each value multiplied with MR rows of x (fp32 FMAs: 2 MR operations per value stay
+// below the vector rate up to 16 rows).  W by rows of r (across): a lane owns 16 bytes of columns, the workgroup's
+// four waves share a range of r, ranges become partial sums for k_finish.
+struct RowsArgs {
+  const void *x, *w;
+  int64_t ldx, ldw;
+  int M, N, K, per, groups;   // per: r values of a workgroup; groups: workgroups along the columns
+  float* part;
+  Epilogue e;
+};
+constexpr int ROWS_MAX_PER = 128;
+
+template <typename T, int MR>
+__global__ __launch_bounds__(256) void k_rows_across(RowsArgs a) {
+  constexpr int V = Vec<T>::N;
+  __shared__ float xs[ROWS_MAX_PER * MR];
+  __shared__ float red[4][64 * V];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int group = blockIdx.x % a.groups, split = blockIdx.x / a.groups;
+  const int k0 = split * a.per, have = min(a.per, a.K - k0);
+  for (int t = threadIdx.x; t < have * MR; t += 256) {
+    const int m = t / have, k = t - m * have;
+    xs[k * MR + m] = m < a.M ? (float)((const T*)a.x)[m * a.ldx + k0 + k] : 0.0f;
+  }
+  __syncthreads();
+  const int col = (group * 64 + lane) * V, n = a.N - col;
+  const T* w = (const T*)a.w + (int64_t)k0 * a.ldw + (n > 0 ? col : 0);
+  float acc[MR][V];
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[m][i] = 0.0f;
+  auto add = [&](int k, const Vec<T>& v) {
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      const float x = xs[k * MR + m];
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[m][i] = fmaf(x, (float)v.v[i], acc[m][i]);
+    }
+  };
+  if (n >= V || n <= 0) {   // lanes behind the last column read the first ones; their sums are not stored
+    const bool wide = a.N >= V;
+    int k = wave;
+    for (; wide && k + 28 < have; k += 32) {
+      Vec<T> v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = load_vec(w + (int64_t)(k + 4 * u) * a.ldw);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) add(k + 4 * u, v[u]);
+    }
+    for (; k < have; k += 4) add(k, load_vec(w + (int64_t)k * a.ldw, wide ? V : a.N));
+  } else {
+    for (int k = wave; k < have; k += 4) add(k, load_vec(w + (int64_t)k * a.ldw, n));
+  }
+#pragma unroll
+  for (int m = 0; m < MR; ++m) {
+    if (m > 0) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i) red[wave][lane * V + i] = acc[m][i];
+    __syncthreads();
+    for (int t = threadIdx.x; t < 64 * V; t += 256) {
+      const int j = group * 64 * V + t;
+      if (m < a.M && j < a.N) a.part[((size_t)split * a.M + m) * a.N + j] = (red[0][t] + red[1][t]) + (red[2][t] + red[3][t]);
+    }
+  }
+}
+
+// W by rows of j (along r): a workgroup owns NR rows of W, its lanes run along r.
+template <typename T, int MR, int NR>
+__global__ __launch_bounds__(256) void k_rows_along(RowsArgs a) {
+  constexpr int V = Vec<T>::N;
+  __shared__ float red[4][MR * NR];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j0 = blockIdx.x * NR;
+  const T* w[NR];
+#pragma unroll
+  for (int j = 0; j < NR; ++j) w[j] = (const T*)a.w + (int64_t)min(j0 + j, a.N - 1) * a.ldw;
+  float acc[MR][NR];
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int j = 0; j < NR; ++j) acc[m][j] = 0.0f;
+  for (int k = threadIdx.x * V; k < a.K; k += 256 * V) {
+    const int n = a.K - k;
+    Vec<T> wv[NR];
+#pragma unroll
+    for (int j = 0; j < NR; ++j) wv[j] = load_vec(w[j] + k, n);
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      const Vec<T> xv = load_vec((const T*)a.x + min(m, a.M - 1) * a.ldx + k, n);
+#pragma unroll
+      for (int j = 0; j < NR; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[m][j] = fmaf((float)xv.v[i], (float)wv[j].v[i], acc[m][j]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+      float s = acc[m][j];
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d, 64);
+      if (lane == 0) red[wave][m * NR + j] = s;
+    }
+  __syncthreads();
+  if (threadIdx.x < MR * NR) {
+    const int m = threadIdx.x / NR, j = j0 + threadIdx.x % NR;
+    if (m < a.M && j < a.N)
+      finish_one<T>(a.e, m, j, (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]));
+  }
+}
+
+// ---- dz = dy act'(pre) and partial column sums of it -------------------------------------------------------------------
+// A lane owns 16 bytes of columns; rows narrower than a wave put several rows into it.
+struct GateArgs {
+  const void *dy, *pre;
+  void* dz;          // null: only the sums
+  float* part;       // [row blocks][N] or null
+  int64_t lddy, ldp, ldz, M, rows_per;
+  int N, lanes, groups, act;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void k_gate(GateArgs a) {
+  constexpr int V = Vec<T>::N;
+  __shared__ float red[256 * V];
+  const int L = a.lanes, sub = threadIdx.x % L, line = threadIdx.x / L, lines = 256 / L;
+  const int group = blockIdx.x % a.groups;
+  const int64_t rb = blockIdx.x / a.groups;
+  const int col = (group * L + sub) * V, n = a.N - col;
+  const int64_t r1 = min(a.M, (rb + 1) * a.rows_per);
+  float s[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) s[i] = 0.0f;
+  if (n > 0) {
+#pragma unroll 4
+    for (int64_t r = rb * a.rows_per + line; r < r1; r += lines) {
+      const Vec<T> g = load_vec((const T*)a.dy + r * a.lddy + col, n);
+      float v[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = (float)g.v[i];
+      if (a.act != DISN_ACT_NONE) {
+        const Vec<T> z = load_vec((const T*)a.pre + r * a.ldp + col, n);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] *= slope((float)z.v[i], a.act);
+      }
+      if (a.dz) {
+        Vec<T> o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o.v[i] = (T)v[i];
+        store_vec((T*)a.dz + r * a.ldz + col, o, n);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] += v[i];
+    }
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = s[i];
+  __syncthreads();
+  for (int t = threadIdx.x; t < L * V; t += 256) {
+    float z = red[t];
+    for (int l = 1; l < lines; ++l) z += red[l * L * V + t];
+    const int j = group * L * V + t;
+    if (j < a.N) a.part[(size_t)rb * a.N + j] = z;
+  }
+}
+
+// ---- host: which kernel, which tile ------------------------------------------------------------------------------------
+enum Kind { K_EMPTY, K_SMALL, K_ROWS, K_TILE };
+struct Product {
+  const void *A, *B;
+  int64_t lda, ldb;
+  bool a_across, b_across;
+  int64_t M, N, K;
+  Epilogue e;
+};
+struct Plan {
+  Kind kind;
+  int tile;            // 128 or 256
+  int splits;
+  int64_t per;
+  size_t bytes;        // of partial sums
+};
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+Plan plan(int type, bool a_across, bool b_across, int64_t M, int64_t N, int64_t K) {
+  Plan p{K_EMPTY, 0, 0, 0, 0};
+  if (M == 0 || N == 0 || K == 0) return p;
+  const int V = type == DISN_F32 ? 4 : 8, KT = type == DISN_F32 ? 16 : 64;
+  if (!a_across && M <= 16 && K * N >= (1 << 20)) {
+    p.kind = K_ROWS;
+    if (!b_across) return p;
+    const int64_t groups = ceil_div(N, 64 * V);
+    int64_t want = ceil_div(1024, groups);
+    p.per = ceil_div(ceil_div(K, want), 32) * 32;
+    if (p.per > ROWS_MAX_PER) p.per = ROWS_MAX_PER;
+    p.splits = (int)ceil_div(K, p.per);
+    p.bytes = (size_t)p.splits * M * N * sizeof(float);
+    return p;
+  }
+  if ((double)M * N * K <= (1 << 27) && ceil_div(M, 16) * ceil_div(N, 16) <= (1 << 20)) {
+    p.kind = K_SMALL;
+    return p;
+  }
+  p.kind = K_TILE;
+  p.tile = ceil_div(M, 256) * ceil_div(N, 256) >= 256 ? 256 : 128;
+  const int64_t tiles = ceil_div(M, p.tile) * ceil_div(N, p.tile);
+  int64_t want = tiles >= 256 ? 1 : 512 / tiles;
+  const int64_t most = ceil_div(K, 4 * KT);
+  if (want > most) want = most;
+  p.per = ceil_div(ceil_div(K, want), KT) * KT;
+  p.splits = (int)ceil_div(K, p.per);
+  p.bytes = p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0;
+  return p;
+}
+
+template <typename T>
+int launch_finish(DisnCtx* ctx, const float* part, int nparts, int64_t M, int64_t N, const Epilogue& e, hipStream_t stream) {
+  if (M == 0 || N == 0) return DISN_OK;
+  const int64_t blocks = ceil_div(M * ceil_div(N, Vec<T>::N), 256);
+  k_finish<T><<<(unsigned)(blocks < 8192 ? blocks : 8192), 256, 0, stream>>>(part, nparts, M, (int)N, e);
+  DISN_HIP(ctx, hipGetLastError());
+  return DISN_OK;
+}
+
+template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN>
+int launch_tile(DisnCtx* ctx, const TileArgs& a, hipStream_t stream) {
+  constexpr int THREADS = WM * WN * 64;
+  constexpr int bytes = 2 * (Operand<T, A_ACROSS, BM, THREADS>::BYTES + Operand<T, B_ACROSS, BN, THREADS>::BYTES);
+  static_assert(bytes <= 160 * 1024, "LDS");
+  auto* kernel = k_tile<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN>;
+  DISN_HIP(ctx, hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  kernel<<<(unsigned)((int64_t)a.mt * a.nt * a.splits), THREADS, bytes, stream>>>(a);
+  DISN_HIP(ctx, hipGetLastError());
+  return DISN_OK;
+}
+template <typename T, bool A_ACROSS, bool B_ACROSS>
+int launch_tile(DisnCtx* ctx, int tile, const TileArgs& a, hipStream_t stream) {
+  return tile == 256 ? launch_tile<T, A_ACROSS, B_ACROSS, 256, 256, 2, 4>(ctx, a, stream)
+                     : launch_tile<T, A_ACROSS, B_ACROSS, 128, 128, 2, 2>(ctx, a, stream);
+}
+
+template <typename T, int MR>
+void launch_rows(const RowsArgs& a, bool b_across, int splits, hipStream_t stream) {
+  if (b_across)
+    k_rows_across<T, MR><<<(unsigned)(a.groups * splits), 256, 0, stream>>>(a);
+  else
+    k_rows_along<T, MR, 4><<<(unsigned)ceil_div(a.N, 4), 256, 0, stream>>>(a);
+}
+
+SmallArgs small_args(const Product& q, const Plan&) {
+  SmallArgs s{};
+  s.A = {q.A, nullptr, q.lda, 0}, s.B = {q.B, nullptr, q.ldb, 0};
+  s.M = (int)q.M, s.N = (int)q.N, s.K = (int)q.K;
+  s.mt = (int)ceil_div(q.M, 16), s.nt = (int)ceil_div(q.N, 16);
+  s.ks = q.K >= 128 ? SMALL_WAVES : 1;
+  s.e = q.e;
+  return s;
+}
+int64_t small_blocks(const SmallArgs& s) { return (int64_t)s.mt * ceil_div(s.nt, SMALL_WAVES / s.ks); }
+
+// one product by its plan; part: plan.bytes of workspace
+template <typename T>
+int run_product(DisnCtx* ctx, const Product& q, const Plan& p, float* part, hipStream_t stream) {
+  if (q.M == 0 || q.N == 0) return DISN_OK;
+  if (p.kind == K_EMPTY) return launch_finish<T>(ctx, nullptr, 0, q.M, q.N, q.e, stream);
+  if (p.kind == K_SMALL) {
+    const SmallArgs s = small_args(q, p);
+    const unsigned blocks = (unsigned)small_blocks(s);
+    if (q.a_across) {
+      // dW beside a large dx: the paired kernel without a dx
+      k_small_backward<T, false><<<blocks, SMALL_WAVES * 64, 0, stream>>>(s, s, 0);
+    } else if (q.b_across) {
+      k_small<T, true><<<blocks, SMALL_WAVES * 64, 0, stream>>>(s);
+    } else {
+      k_small<T, false><<<blocks, SMALL_WAVES * 64, 0, stream>>>(s);
+    }
+    DISN_HIP(ctx, hipGetLastError());
+    return DISN_OK;
+  }
+  if (p.kind == K_ROWS) {
+    RowsArgs r{q.A, q.B, q.lda, q.ldb, (int)q.M, (int)q.N, (int)q.K, (int)p.per, (int)ceil_div(q.N, 64 * Vec<T>::N), part, q.e};
+    if (q.M == 1) launch_rows<T, 1>(r, q.b_across, p.splits, stream);
+    else if (q.M <= 4) launch_rows<T, 4>(r, q.b_across, p.splits, stream);
+    else launch_rows<T, 16>(r, q.b_across, p.splits, stream);
+    DISN_HIP(ctx, hipGetLastError());
+    return q.b_across ? launch_finish<T>(ctx, part, p.splits, q.M, q.N, q.e, stream) : DISN_OK;
+  }
+  TileArgs t{q.A, q.B, q.lda, q.ldb, (int)q.M, (int)q.N, q.K, p.per, (int)ceil_div(q.M, p.tile), (int)ceil_div(q.N, p.tile), p.splits,
+             part, q.e};
+  if (q.a_across) DISN_TRY((launch_tile<T, true, true>(ctx, p.tile, t, stream)));
+  else if (q.b_across) DISN_TRY((launch_tile<T, false, true>(ctx, p.tile, t, stream)));
+  else DISN_TRY((launch_tile<T, false, false>(ctx, p.tile, t, stream)));
+  return p.splits > 1 ? launch_finish<T>(ctx, part, p.splits, q.M, q.N, q.e, stream) : DISN_OK;
+}
+
+// ---- host: arguments -----------------------------------------------------------------------------------------------------
+int check_linear(DisnCtx* ctx, const DisnLinear* a) {
+  const char* f = "disn_linear";
+  if (!a) return disn_fail(ctx, DISN_E_ARG, "%s: null arguments", f);
+  if (!dense_type_ok(a->type) || a->act < DISN_ACT_NONE || a->act > DISN_ACT_SILU || a->w_nk < 0 || a->w_nk > 1 || a->reserved)
+    return disn_fail(ctx, DISN_E_ARG, "%s: bad type %d, act %d, w_nk %d or reserved field", f, a->type, a->act, a->w_nk);
+  if (!dense_size_ok(a->m) || !dense_size_ok(a->n) || !dense_size_ok(a->k))
+    return disn_fail(ctx, DISN_E_ARG, "%s: sizes %lld, %lld, %lld", f, (long long)a->m, (long long)a->n, (long long)a->k);
+  const size_t s = dense_type_size(a->type);
+  if (a->m == 0 || a->n == 0) return DISN_OK;
+  if (!dense_matrix_ok(a->x, a->m, a->k, a->ldx, s, true) ||
+      !dense_matrix_ok(a->w, a->w_nk ? a->n : a->k, a->w_nk ? a->k : a->n, a->ldw, s, true) ||
+      !dense_matrix_ok(a->y, a->m, a->n, a->ldy, s, false) || (a->residual && !dense_matrix_ok(a->residual, a->m, a->n, a->ldr, s, true)) ||
+      (a->pre && !dense_matrix_ok(a->pre, a->m, a->n, a->ldp, s, false)))
+    return disn_fail(ctx, DISN_E_ARG, "%s: a matrix is null, misaligned or has a bad row distance", f);
+  if (!dense_aligned(a->bias, s)) return disn_fail(ctx, DISN_E_ARG, "%s: bias is misaligned", f);
+  return DISN_OK;
+}
+
+int check_linear_grad(DisnCtx* ctx, const DisnLinearGrad* a) {
+  const char* f = "disn_linear_backward";
+  if (!a) return disn_fail(ctx, DISN_E_ARG, "%s: null arguments", f);
+  if (!dense_type_ok(a->type) || a->act < DISN_ACT_NONE || a->act > DISN_ACT_SILU || a->w_nk < 0 || a->w_nk > 1 || a->reserved)
+    return disn_fail(ctx, DISN_E_ARG, "%s: bad type %d, act %d, w_nk %d or reserved field", f, a->type, a->act, a->w_nk);
+  if (!dense_size_ok(a->m) || !dense_size_ok(a->n) || !dense_size_ok(a->k))
+    return disn_fail(ctx, DISN_E_ARG, "%s: sizes %lld, %lld, %lld", f, (long long)a->m, (long long)a->n, (long long)a->k);
+  const size_t s = dense_type_size(a->type);
+  const int64_t wr = a->w_nk ? a->n : a->k, wc = a->w_nk ? a->k : a->n;
+  if ((a->act == DISN_ACT_NONE) != !a->pre && a->m && a->n)
+    return disn_fail(ctx, DISN_E_ARG, "%s: pre belongs to an activation (act %d)", f, a->act);
+  if (!dense_matrix_ok(a->dy, a->m, a->n, a->lddy, s, true) || (a->pre && !dense_matrix_ok(a->pre, a->m, a->n, a->ldp, s, true)) ||
+      (a->dx && !dense_matrix_ok(a->dx, a->m, a->k, a->lddx, s, false)) || (a->dw && !dense_matrix_ok(a->dw, wr, wc, a->lddw, s, false)) ||
+      (a->dx && !dense_matrix_ok(a->w, wr, wc, a->ldw, s, true)) || (a->dw && !dense_matrix_ok(a->x, a->m, a->k, a->ldx, s, true)))
+    return disn_fail(ctx, DISN_E_ARG, "%s: a matrix is null, misaligned or has a bad row distance", f);
+  if (!dense_aligned(a->db, s)) return disn_fail(ctx, DISN_E_ARG, "%s: db is misaligned", f);
+  return DISN_OK;
+}
+
+Product forward_product(const DisnLinear* a) {
+  return {a->x, a->w, a->ldx, a->ldw, false, a->w_nk == 0, a->m, a->n, a->k,
+          {a->bias, a->residual, a->pre, a->y, a->ldr, a->ldp, a->ldy, a->act}};
+}
+
+// The backward pass of one call: small ones are one launch; others write dz once (act != none), then two products.
+struct GradPlan {
+  bool small;
+  Plan dx, dw;
+  int64_t ldz, gate_blocks, gate_rows;
+  int gate_lanes, gate_groups;
+  size_t off_sums, off_part, bytes;   // workspace: dz, partial column sums, partial products
+};
+size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+GradPlan plan_backward(const DisnLinearGrad* a) {
+  GradPlan g{};
+  const size_t s = dense_type_size(a->type);
+  if (a->dx) g.dx = plan(a->type, false, a->w_nk != 0, a->m, a->k, a->n);
+  if (a->dw) g.dw = a->w_nk ? plan(a->type, true, true, a->n, a->k, a->m) : plan(a->type, true, true, a->k, a->n, a->m);
+  g.small = a->dw && g.dw.kind == K_SMALL && (!a->dx || g.dx.kind == K_SMALL);
+  if (g.small) return g;
+  const int V = (int)(16 / s);
+  g.ldz = ceil_div(a->n, V) * V;
+  g.gate_lanes = 1;
+  while (g.gate_lanes < 64 && g.gate_lanes * V < a->n) g.gate_lanes *= 2;
+  g.gate_groups = (int)ceil_div(a->n, g.gate_lanes * V);
+  if (g.gate_groups < 1) g.gate_groups = 1;
+  // row blocks: about 1024 workgroups, at least 8 rows a thread
+  const int64_t lines = 256 / g.gate_lanes;
+  int64_t blocks = ceil_div(1024, g.gate_groups);
+  if (blocks > ceil_div(a->m, lines * 8)) blocks = ceil_div(a->m, lines * 8);
+  if (blocks < 1) blocks = 1;
+  g.gate_rows = ceil_div(a->m, blocks);
+  g.gate_blocks = a->m ? ceil_div(a->m, g.gate_rows) : 0;
+  size_t at = 0;
+  if (a->act != DISN_ACT_NONE && (a->dx || a->dw)) at += align256((size_t)a->m * g.ldz * s);
+  g.off_sums = at;
+  if (a->db) at += align256((size_t)g.gate_blocks * a->n * sizeof(float));
+  g.off_part = at;
+  at += g.dx.bytes > g.dw.bytes ? g.dx.bytes : g.dw.bytes;
+  g.bytes = at;
+  return g;
+}
+
+template <typename T>
+int run_backward(DisnCtx* ctx, const DisnLinearGrad* a, const GradPlan& g, char* ws, hipStream_t stream) {
+  const bool gated = a->act != DISN_ACT_NONE;
+  const void* dz = a->dy;
+  int64_t ldz = a->lddy;
+  if (!g.small) {
+    const bool write = gated && (a->dx || a->dw);
+    if (a->n && a->m && (write || a->db)) {
+      GateArgs k{a->dy, a->pre, write ? ws : nullptr, a->db ? (float*)(ws + g.off_sums) : nullptr, a->lddy, a->ldp, g.ldz, a->m,
+                 g.gate_rows, (int)a->n, g.gate_lanes, g.gate_groups, a->act};
+      k_gate<T><<<(unsigned)(g.gate_groups * g.gate_blocks), 256, 0, stream>>>(k);
+      DISN_HIP(ctx, hipGetLastError());
+    }
+    if (a->db && a->n) {
+      k_sum_partials<T><<<(unsigned)ceil_div(a->n, 16), 256, 0, stream>>>((const float*)(ws + g.off_sums), (int)g.gate_blocks, a->n, a->n,
+                                                                          (T*)a->db, (T*)nullptr);
+      DISN_HIP(ctx, hipGetLastError());
+    }
+    if (write) dz = ws, ldz = g.ldz;
+  }
+  Product dx{dz, a->w, ldz, a->ldw, false, a->w_nk != 0, a->m, a->k, a->n, {nullptr, nullptr, nullptr, a->dx, 0, 0, a->lddx, DISN_ACT_NONE}};
+  Product dw{a->x, dz, a->ldx, ldz, true, true, a->k, a->n, a->m, {nullptr, nullptr, nullptr, a->dw, 0, 0, a->lddw, DISN_ACT_NONE}};
+  if (a->w_nk) dw = {dz, a->x, ldz, a->ldx, true, true, a->n, a->k, a->m, dw.e};
+  if (!g.small) {
+    if (a->dx) DISN_TRY(run_product<T>(ctx, dx, g.dx, (float*)(ws + g.off_part), stream));
+    if (a->dw) DISN_TRY(run_product<T>(ctx, dw, g.dw, (float*)(ws + g.off_part), stream));
+    return DISN_OK;
+  }
+  SmallArgs sx = small_args(dx, g.dx), sw = small_args(dw, g.dw);
+  sx.act = sw.act = a->act;
+  sx.A.gate = a->pre, sx.A.ldg = a->ldp;
+  SmallOperand& of = a->w_nk ? sw.A : sw.B;
+  of.gate = a->pre, of.ldg = a->ldp;
+  sw.rsum = a->db, sw.rsum_of_a = a->w_nk;
+  const int64_t first = a->dx ? small_blocks(sx) : 0, blocks = first + small_blocks(sw);
+  if (a->w_nk)
+    k_small_backward<T, true><<<(unsigned)blocks, SMALL_WAVES * 64, 0, stream>>>(sx, sw, (int)first);
+  else
+    k_small_backward<T, false><<<(unsigned)blocks, SMALL_WAVES * 64, 0, stream>>>(sx, sw, (int)first);
+  DISN_HIP(ctx, hipGetLastError());
+  return DISN_OK;
+}
+
+}  // namespace
+
+extern "C" int disn_linear_workspace(DisnCtx* ctx, const DisnLinear* a, size_t* bytes) {
+  if (!ctx) return DISN_E_ARG;
+  if (!bytes) return disn_fail(ctx, DISN_E_ARG, "disn_linear_workspace: null result");
+  DISN_TRY(check_linear(ctx, a));
+  *bytes = plan(a->type, false, a->w_nk == 0, a->m, a->n, a->k).bytes;
+  return DISN_OK;
+}
+
+extern "C" int disn_linear(DisnCtx* ctx, const DisnLinear* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!ctx) return DISN_E_ARG;
+  DISN_TRY(check_linear(ctx, a));
+  const Plan p = plan(a->type, false, a->w_nk == 0, a->m, a->n, a->k);
+  if (p.bytes && (!workspace || !dense_aligned(workspace, 16) || workspace_bytes < p.bytes))
+    return disn_fail(ctx, DISN_E_ARG, "disn_linear: needs %zu bytes of 16-byte aligned workspace", p.bytes);
+  DISN_HIP(ctx, hipSetDevice(ctx->device));
+  return dense_dispatch(a->type, [&](auto t) {
+    return run_product<decltype(t)>(ctx, forward_product(a), p, (float*)workspace, (hipStream_t)stream);
+  });
+}
+
+extern "C" int disn_linear_backward_workspace(DisnCtx* ctx, const DisnLinearGrad* a, size_t* bytes) {
+  if (!ctx) return DISN_E_ARG;
+  if (!bytes) return disn_fail(ctx, DISN_E_ARG, "disn_linear_backward_workspace: null result");
+  DISN_TRY(check_linear_grad(ctx, a));
+  *bytes = plan_backward(a).bytes;
+  return DISN_OK;
+}
+
+extern "C" int disn_linear_backward(DisnCtx* ctx, const DisnLinearGrad* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!ctx) return DISN_E_ARG;
+  DISN_TRY(check_linear_grad(ctx, a));
+  const GradPlan g = plan_backward(a);
+  if (g.bytes && (!workspace || !dense_aligned(workspace, 16) || workspace_bytes < g.bytes))
+    return disn_fail(ctx, DISN_E_ARG, "disn_linear_backward: needs %zu bytes of 16-byte aligned workspace", g.bytes);
+  DISN_HIP(ctx, hipSetDevice(ctx->device));
+  return dense_dispatch(a->type, [&](auto t) {
+    return run_backward<decltype(t)>(ctx, a, g, (char*)workspace, (hipStream_t)stream);
+  });
+}

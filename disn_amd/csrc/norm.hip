@@ -1,0 +1,344 @@
+// norm.hip -- layer norm over the rows of a matrix, forward and backward (include/disn.h).
+//
+// Forward, per row:   mean = sum x / d;  var = sum (x - mean)^2 / d;  rstd = 1 / sqrt(var + eps);
+//                     y = (x - mean) rstd g + b
+// Backward, per row:  h = (x - mean) rstd;  t = dy g;  dx = rstd (t - avg(t) - h avg(t h)) + residual
+//            columns: dg = sum over rows of dy h;  db = sum over rows of dy
+//
+// Both are bound by memory: every value is read once and written once.  A group of G threads holds a whole row in
+// registers, E values a thread in 16-byte pieces, so the variance is the sum of squared distances from the mean that
+// is already known (not a difference of two large sums) and costs no second read.  G = 16 / 64: rows inside a wave
+// (no barrier, sums by lane exchange), 256 / 1024: a row per workgroup.  The backward pass walks over rows with a
+// fixed set of workgroups; a thread meets the same columns in every row and sums their dg, db in registers; the
+// workgroups' sums are added in order by a second kernel.
+#include "dense.h"
+
+namespace {
+
+struct NormArgs {
+  const void *x, *weight, *bias, *dy, *residual;
+  const float *mean_in, *rstd_in;
+  void *y, *dweight, *dbias;
+  float *mean, *rstd, *part;
+  int64_t ldx, ldy, lddy, ldr;
+  int64_t rows;
+  int d;
+  float eps;
+};
+
+// sum over the G threads of a row's group; lds: two slots of 16 floats, used in turn (a slot is rewritten two sums
+// later, behind the other sum's barrier)
+template <int G>
+__device__ __forceinline__ float group_sum(float v, float (*lds)[16], int slot) {
+#pragma unroll
+  for (int m = (G < 64 ? G : 64) / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+  if constexpr (G > 64) {
+    if ((threadIdx.x & 63) == 0) lds[slot][threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = lds[slot][0];
+#pragma unroll
+    for (int i = 1; i < G / 64; ++i) v += lds[slot][i];
+  }
+  return v;
+}
+
+// column of the piece p that a thread of a group holds, and how many of its values lie inside the row
+template <typename T, int G>
+__device__ __forceinline__ int piece_col(int t, int p) { return (p * G + t) * Vec<T>::N; }
+
+template <typename T, int E>
+__device__ __forceinline__ void widen(const Vec<T> (&in)[E / Vec<T>::N], float (&out)[E]) {
+#pragma unroll
+  for (int i = 0; i < E; ++i) out[i] = (float)in[i / Vec<T>::N].v[i % Vec<T>::N];
+}
+
+template <typename T, int G, int E>
+__device__ __forceinline__ void load_row(const T* row, int t, int d, Vec<T> (&out)[E / Vec<T>::N]) {
+#pragma unroll
+  for (int p = 0; p < E / Vec<T>::N; ++p) {
+    const int c = piece_col<T, G>(t, p);
+    out[p] = load_vec(row + (c < d ? c : 0), c < d ? d - c : 0);
+  }
+}
+
+template <typename T, int G, int E>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm(NormArgs a) {
+  constexpr int N = Vec<T>::N, P = E / N, B = G < 256 ? 256 : G;
+  __shared__ float lds[2][16];
+  const int t = threadIdx.x % G, d = a.d;
+  float w[E], b[E];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int c = piece_col<T, G>(t, p), n = c < d ? d - c : 0;
+    const Vec<T> wv = a.weight ? load_vec((const T*)a.weight + (n ? c : 0), n) : Vec<T>{};
+    const Vec<T> bv = a.bias ? load_vec((const T*)a.bias + (n ? c : 0), n) : Vec<T>{};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      w[p * N + i] = a.weight ? (float)wv.v[i] : 1.0f;
+      b[p * N + i] = a.bias ? (float)bv.v[i] : 0.0f;
+    }
+  }
+  const float inv = 1.0f / (float)d;
+  for (int64_t row = (int64_t)blockIdx.x * (B / G) + threadIdx.x / G; row < a.rows; row += (int64_t)gridDim.x * (B / G)) {
+    Vec<T> xv[P];
+    load_row<T, G, E>((const T*)a.x + row * a.ldx, t, d, xv);
+    float x[E];
+    widen<T, E>(xv, x);
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) s += x[i];   // places behind the row hold 0
+    const float mean = group_sum<G>(s, lds, 0) * inv;
+    s = 0.0f;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float c = piece_col<T, G>(t, p) + i < d ? x[p * N + i] - mean : 0.0f;
+        x[p * N + i] = c;
+        s = fmaf(c, c, s);
+      }
+    const float rstd = 1.0f / sqrtf(group_sum<G>(s, lds, 1) * inv + a.eps);
+    if (t == 0) {
+      if (a.mean) a.mean[row] = mean;
+      if (a.rstd) a.rstd[row] = rstd;
+    }
+    T* y = (T*)a.y + row * a.ldy;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int c = piece_col<T, G>(t, p);
+      if (c >= d) break;
+      Vec<T> o;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o.v[i] = (T)fmaf(x[p * N + i] * rstd, w[p * N + i], b[p * N + i]);
+      store_vec(y + c, o, d - c);
+    }
+  }
+}
+
+template <typename T, int G, int E>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm_backward(NormArgs a) {
+  constexpr int N = Vec<T>::N, P = E / N, B = G < 256 ? 256 : G;
+  __shared__ float lds[2][16];
+  const int t = threadIdx.x % G, d = a.d;
+  float w[E], dg[E], db[E];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int c = piece_col<T, G>(t, p), n = c < d ? d - c : 0;
+    const Vec<T> wv = a.weight ? load_vec((const T*)a.weight + (n ? c : 0), n) : Vec<T>{};
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[p * N + i] = a.weight ? (float)wv.v[i] : 1.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) dg[i] = db[i] = 0.0f;
+  const float inv = 1.0f / (float)d;
+  for (int64_t row = (int64_t)blockIdx.x * (B / G) + threadIdx.x / G; row < a.rows; row += (int64_t)gridDim.x * (B / G)) {
+    Vec<T> xv[P], gv[P], rv[P];
+    load_row<T, G, E>((const T*)a.x + row * a.ldx, t, d, xv);
+    load_row<T, G, E>((const T*)a.dy + row * a.lddy, t, d, gv);
+    if (a.y && a.residual) load_row<T, G, E>((const T*)a.residual + row * a.ldr, t, d, rv);
+    const float mean = a.mean_in[row], rstd = a.rstd_in[row];
+    float h[E], g[E], s1 = 0.0f, s2 = 0.0f;
+    widen<T, E>(xv, h);
+    widen<T, E>(gv, g);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      h[i] = (h[i] - mean) * rstd;   // places behind the row: finite or not, their g is 0 ...
+      const bool in = piece_col<T, G>(t, i / N) + i % N < d;
+      if (!in) h[i] = 0.0f;          // ... and a NaN of the row's statistics must not meet it
+      dg[i] = fmaf(g[i], h[i], dg[i]);
+      db[i] += g[i];
+      g[i] *= w[i];
+      s1 += g[i];
+      s2 = fmaf(g[i], h[i], s2);
+    }
+    if (!a.y) continue;
+    s1 = group_sum<G>(s1, lds, 0) * inv;
+    s2 = group_sum<G>(s2, lds, 1) * inv;
+    T* dx = (T*)a.y + row * a.ldy;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int c = piece_col<T, G>(t, p);
+      if (c >= d) break;
+      Vec<T> o;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int e = p * N + i;
+        float v = rstd * (g[e] - s1 - h[e] * s2);
+        if (a.residual) v += (float)rv[p].v[i];
+        o.v[i] = (T)v;
+      }
+      store_vec(dx + c, o, d - c);
+    }
+  }
+  if (!a.dweight && !a.dbias) return;
+  // the workgroup's sums: groups of one workgroup through LDS in group order, then out (one workgroup) or partial sums
+  constexpr int K = B / G;
+  __shared__ float red[K > 1 ? B * E : 1];
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    float(&v)[E] = which ? db : dg;
+    if constexpr (K > 1) {
+      if (which) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < E; ++i) red[threadIdx.x * E + i] = v[i];
+      __syncthreads();
+      if (threadIdx.x < G) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          float s = red[threadIdx.x * E + i];
+          for (int k = 1; k < K; ++k) s += red[(k * G + threadIdx.x) * E + i];
+          v[i] = s;
+        }
+      }
+    }
+    if (threadIdx.x < G) {
+      T* out = (T*)(which ? a.dbias : a.dweight);
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int c = piece_col<T, G>(t, p) + i;
+          if (c >= d) continue;
+          if (gridDim.x == 1) {
+            if (out) out[c] = (T)v[p * N + i];
+          } else {
+            a.part[(size_t)blockIdx.x * 2 * d + (size_t)which * d + c] = v[p * N + i];
+          }
+        }
+    }
+  }
+}
+
+// group size and values per thread for a row of d values.  Small rows share a wave; up to 1024 values a wave
+// holds a row without barriers; the row is spread wider before a thread holds more than 16 values.
+struct NormShape {
+  int group, per_thread;
+};
+NormShape norm_shape(int64_t d) {
+  if (d <= 128) return {16, 8};
+  if (d <= 512) return {64, 8};
+  if (d <= 1024) return {64, 16};
+  if (d <= 2048) return {256, 8};
+  if (d <= 4096) return {256, 16};
+  return {1024, 8};
+}
+// workgroups of the backward pass: four of 256 threads a CU (one of 1024), each at least four rows a group, so
+// that its partial sums (2 d floats) stay small beside the rows it reads
+int64_t norm_backward_grid(const NormShape& s, int64_t rows) {
+  const int64_t per = s.group < 256 ? 256 / s.group : 1;
+  const int64_t most = s.group == 1024 ? 256 : 1024, want = (rows + per * 4 - 1) / (per * 4);
+  return want < 1 ? 1 : want < most ? want : most;
+}
+
+template <typename T, int G, int E>
+void launch_norm(bool backward, const NormArgs& a, int64_t grid, hipStream_t stream) {
+  constexpr int B = G < 256 ? 256 : G;
+  if (backward)
+    k_layer_norm_backward<T, G, E><<<(unsigned)grid, B, 0, stream>>>(a);
+  else
+    k_layer_norm<T, G, E><<<(unsigned)grid, B, 0, stream>>>(a);
+}
+template <typename T>
+void launch_norm(const NormShape& s, bool backward, const NormArgs& a, int64_t grid, hipStream_t stream) {
+  if (s.group == 16) launch_norm<T, 16, 8>(backward, a, grid, stream);
+  else if (s.group == 64 && s.per_thread == 8) launch_norm<T, 64, 8>(backward, a, grid, stream);
+  else if (s.group == 64) launch_norm<T, 64, 16>(backward, a, grid, stream);
+  else if (s.group == 256 && s.per_thread == 8) launch_norm<T, 256, 8>(backward, a, grid, stream);
+  else if (s.group == 256) launch_norm<T, 256, 16>(backward, a, grid, stream);
+  else launch_norm<T, 1024, 8>(backward, a, grid, stream);
+}
+
+int check_norm(DisnCtx* ctx, const DisnLayerNorm* a) {
+  const char* f = "disn_layer_norm";
+  if (!a) return disn_fail(ctx, DISN_E_ARG, "%s: null arguments", f);
+  if (!dense_type_ok(a->type) || a->reserved) return disn_fail(ctx, DISN_E_ARG, "%s: bad type %d or reserved field", f, a->type);
+  if (!dense_size_ok(a->rows) || a->d < 1 || a->d > DISN_LAYER_NORM_MAX)
+    return disn_fail(ctx, DISN_E_ARG, "%s: %lld rows of %lld (want d in 1..%d)", f, (long long)a->rows, (long long)a->d, DISN_LAYER_NORM_MAX);
+  if (!(a->eps >= 0.0) || a->eps > 3e38) return disn_fail(ctx, DISN_E_ARG, "%s: eps must be a finite number >= 0", f);
+  const size_t s = dense_type_size(a->type);
+  if (!dense_matrix_ok(a->x, a->rows, a->d, a->ldx, s, true) || !dense_matrix_ok(a->y, a->rows, a->d, a->ldy, s, false))
+    return disn_fail(ctx, DISN_E_ARG, "%s: x or y is null, misaligned or has a bad row distance", f);
+  if (!dense_aligned(a->weight, s) || !dense_aligned(a->bias, s) || !dense_aligned(a->mean, 4) || !dense_aligned(a->rstd, 4))
+    return disn_fail(ctx, DISN_E_ARG, "%s: a vector is misaligned", f);
+  return DISN_OK;
+}
+
+int check_norm_grad(DisnCtx* ctx, const DisnLayerNormGrad* a) {
+  const char* f = "disn_layer_norm_backward";
+  if (!a) return disn_fail(ctx, DISN_E_ARG, "%s: null arguments", f);
+  if (!dense_type_ok(a->type) || a->reserved) return disn_fail(ctx, DISN_E_ARG, "%s: bad type %d or reserved field", f, a->type);
+  if (!dense_size_ok(a->rows) || a->d < 1 || a->d > DISN_LAYER_NORM_MAX)
+    return disn_fail(ctx, DISN_E_ARG, "%s: %lld rows of %lld (want d in 1..%d)", f, (long long)a->rows, (long long)a->d, DISN_LAYER_NORM_MAX);
+  const size_t s = dense_type_size(a->type);
+  if (!dense_matrix_ok(a->x, a->rows, a->d, a->ldx, s, true) || !dense_matrix_ok(a->dy, a->rows, a->d, a->lddy, s, true) ||
+      (a->dx && !dense_matrix_ok(a->dx, a->rows, a->d, a->lddx, s, false)) ||
+      (a->residual && !dense_matrix_ok(a->residual, a->rows, a->d, a->ldr, s, true)))
+    return disn_fail(ctx, DISN_E_ARG, "%s: a matrix is null, misaligned or has a bad row distance", f);
+  if (a->rows && (!a->mean || !a->rstd)) return disn_fail(ctx, DISN_E_ARG, "%s: mean and rstd of the forward pass are needed", f);
+  if (!dense_aligned(a->weight, s) || !dense_aligned(a->dweight, s) || !dense_aligned(a->dbias, s) || !dense_aligned(a->mean, 4) ||
+      !dense_aligned(a->rstd, 4))
+    return disn_fail(ctx, DISN_E_ARG, "%s: a vector is misaligned", f);
+  return DISN_OK;
+}
+
+size_t norm_grad_workspace(const DisnLayerNormGrad* a) {
+  if (!a->dweight && !a->dbias) return 0;
+  const int64_t grid = norm_backward_grid(norm_shape(a->d), a->rows);
+  return grid == 1 ? 0 : (size_t)grid * 2 * a->d * sizeof(float);
+}
+
+}  // namespace
+
+extern "C" int disn_layer_norm(DisnCtx* ctx, const DisnLayerNorm* a, void* stream_) {
+  if (!ctx) return DISN_E_ARG;
+  DISN_TRY(check_norm(ctx, a));
+  if (a->rows == 0) return DISN_OK;
+  DISN_HIP(ctx, hipSetDevice(ctx->device));
+  NormArgs k{};
+  k.x = a->x, k.weight = a->weight, k.bias = a->bias, k.y = a->y, k.mean = a->mean, k.rstd = a->rstd;
+  k.ldx = a->ldx, k.ldy = a->ldy, k.rows = a->rows, k.d = (int)a->d, k.eps = (float)a->eps;
+  const NormShape s = norm_shape(a->d);
+  const int64_t per = s.group < 256 ? 256 / s.group : 1, want = (a->rows + per - 1) / per, most = s.group == 1024 ? 512 : 2048;
+  dense_dispatch(a->type, [&](auto t) {
+    launch_norm<decltype(t)>(s, false, k, want < most ? want : most, (hipStream_t)stream_);
+    return 0;
+  });
+  DISN_HIP(ctx, hipGetLastError());
+  return DISN_OK;
+}
+
+extern "C" int disn_layer_norm_backward_workspace(DisnCtx* ctx, const DisnLayerNormGrad* a, size_t* bytes) {
+  if (!ctx) return DISN_E_ARG;
+  if (!bytes) return disn_fail(ctx, DISN_E_ARG, "disn_layer_norm_backward_workspace: null result");
+  DISN_TRY(check_norm_grad(ctx, a));
+  *bytes = norm_grad_workspace(a);
+  return DISN_OK;
+}
+
+extern "C" int disn_layer_norm_backward(DisnCtx* ctx, const DisnLayerNormGrad* a, void* workspace, size_t workspace_bytes,
+                                        void* stream_) {
+  if (!ctx) return DISN_E_ARG;
+  DISN_TRY(check_norm_grad(ctx, a));
+  if (!a->dx && !a->dweight && !a->dbias) return DISN_OK;
+  const size_t need = norm_grad_workspace(a);
+  if (need && (!workspace || !dense_aligned(workspace, 16) || workspace_bytes < need))
+    return disn_fail(ctx, DISN_E_ARG, "disn_layer_norm_backward: needs %zu bytes of 16-byte aligned workspace", need);
+  DISN_HIP(ctx, hipSetDevice(ctx->device));
+  hipStream_t stream = (hipStream_t)stream_;
+  NormArgs k{};
+  k.x = a->x, k.dy = a->dy, k.mean_in = a->mean, k.rstd_in = a->rstd, k.weight = a->weight, k.residual = a->residual;
+  k.y = a->dx, k.dweight = a->dweight, k.dbias = a->dbias, k.part = (float*)workspace;
+  k.ldx = a->ldx, k.lddy = a->lddy, k.ldr = a->ldr, k.ldy = a->lddx, k.rows = a->rows, k.d = (int)a->d;
+  const NormShape s = norm_shape(a->d);
+  const int64_t grid = norm_backward_grid(s, a->rows);   // without rows one workgroup writes the empty sums
+  dense_dispatch(a->type, [&](auto t) {
+    using T = decltype(t);
+    launch_norm<T>(s, true, k, grid, stream);
+    if (need)
+      k_sum_partials<T><<<(unsigned)((2 * a->d + 15) / 16), 256, 0, stream>>>(k.part, (int)grid, 2 * a->d, a->d, (T*)a->dweight,
+                                                                              (T*)a->dbias);
+    return 0;
+  });
+  DISN_HIP(ctx, hipGetLastError());
+  return DISN_OK;
+}

@@ -176,6 +176,121 @@ int disn_vgg_set_weights(DisnCtx* ctx, int slot, const DisnVggWeights* w);
 int disn_vgg_forward(DisnCtx* ctx, int slot, const float* img, int img_h, int img_w, float* const feat_maps[5],
                      float* global_feat, void* stream);
 
+/* ---- dense layer and layer norm, forward and backward ------------------- */
+/* Free-standing building blocks of point-wise networks (no counterpart as such in the reference, whose graph builds
+ * every 1x1 convolution and fully connected layer from matmul + bias_add + relu, models/sdfnet.py:69-92,
+ * models/posenet_old.py:104-142, and has no norm): for decoders of other widths, residual blocks and the training of
+ * either.  Common rules:
+ *  - every tensor of a call has the same type; statistics, sums and partial results are fp32, a result is rounded once
+ *  - matrices are rows of contiguous values, `ld*` values apart (ld >= the row's length; inputs may have ld = 0: one
+ *    row for all).  Any base address that fits the type, any size and any ld are allowed; sizes up to 2^30
+ *  - a size of zero is fine: an empty output is not written, a sum over nothing is 0
+ *  - an output must not overlap any other argument.  One exception: y of disn_linear may be the residual itself
+ *    (same address and ld)
+ *  - the workspace (DEVICE, 16-byte aligned, any contents, free again when the stream has passed the call) belongs to
+ *    the caller: its size comes from the *_workspace call on the same arguments (0: may be NULL).  The calls allocate
+ *    nothing, keep nothing and clear nothing through the runtime, so they can be captured into graphs; two graphs or
+ *    streams that may run at the same time need a workspace each
+ *  - results do not depend on the run: fixed summation orders, no atomics */
+#define DISN_F32 0
+#define DISN_BF16 1
+#define DISN_F16 2
+#define DISN_ACT_NONE 0
+#define DISN_ACT_RELU 1
+#define DISN_ACT_GELU 2 /* z (1 + erf(z / sqrt 2)) / 2 */
+#define DISN_ACT_SILU 3 /* z / (1 + exp(-z)) */
+
+/* z = x W + bias;  y = act(z) + residual.
+ *   x [m][k];  w: w_nk = 0 rows of outputs [k][n] (the layout of every weight in this header), 1 rows of inputs [n][k]
+ *   bias [n] or NULL;  residual [m][n] or NULL;  y [m][n];  pre [m][n] or NULL: receives z, for the backward pass
+ * fp32: products as exact in total as an fp32 FMA chain (see csrc/linear.hip), infinities and NaN as in one. */
+typedef struct DisnLinear {
+  int32_t type, act, w_nk, reserved; /* reserved = 0 */
+  int64_t m, n, k;
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  const void* bias;
+  const void* residual;
+  int64_t ldr;
+  void* y;
+  int64_t ldy;
+  void* pre;
+  int64_t ldp;
+} DisnLinear;
+int disn_linear_workspace(DisnCtx* ctx, const DisnLinear* a, size_t* bytes);
+int disn_linear(DisnCtx* ctx, const DisnLinear* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of disn_linear: dz = dy act'(pre);  dx = dz W^T;  dw = x^T dz;  db = sum of dz over the rows.
+ *   dy [m][n] (also the gradient of the residual);  pre [m][n]: z as disn_linear returned it, NULL with
+ *   DISN_ACT_NONE; for DISN_ACT_RELU any tensor that is positive where z is does, y of a call without residual too
+ *   dx [m][k], dw (layout w_nk, like w), db [n]: NULL = not wanted; w may be NULL without dx, x without dw
+ * act'(0) of relu is 0; where pre is NaN, dz is NaN.  16-bit types: dz is rounded to the type before the two
+ * products (they take 16-bit operands) unless act is none. */
+typedef struct DisnLinearGrad {
+  int32_t type, act, w_nk, reserved; /* reserved = 0 */
+  int64_t m, n, k;
+  const void* dy;
+  int64_t lddy;
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  const void* pre;
+  int64_t ldp;
+  void* dx;
+  int64_t lddx;
+  void* dw;
+  int64_t lddw;
+  void* db;
+} DisnLinearGrad;
+int disn_linear_backward_workspace(DisnCtx* ctx, const DisnLinearGrad* a, size_t* bytes);
+int disn_linear_backward(DisnCtx* ctx, const DisnLinearGrad* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* y = (x - mean) rstd weight + bias per row;  mean = sum x / d, rstd = 1 / sqrt(sum (x - mean)^2 / d + eps).
+ *   x, y [rows][d], 1 <= d <= DISN_LAYER_NORM_MAX;  weight, bias [d] or NULL (1 and 0)
+ *   mean, rstd: fp32 [rows] or NULL.  A row that holds an infinity or a NaN gives NaN in all of its values. */
+#define DISN_LAYER_NORM_MAX 8192
+typedef struct DisnLayerNorm {
+  int32_t type, reserved; /* reserved = 0 */
+  int64_t rows, d;
+  const void* x;
+  int64_t ldx;
+  const void* weight;
+  const void* bias;
+  double eps; /* >= 0 */
+  void* y;
+  int64_t ldy;
+  float* mean;
+  float* rstd;
+} DisnLayerNorm;
+int disn_layer_norm(DisnCtx* ctx, const DisnLayerNorm* a, void* stream);
+
+/* Gradients of disn_layer_norm: h = (x - mean) rstd;  t = dy weight;
+ * dx = rstd (t - avg(t) - h avg(t h)) + residual, avg over the row;  dweight = sum of dy h, dbias = sum of dy over the rows.
+ *   residual [rows][d] or NULL: the gradient that reaches x past the norm;  mean, rstd as disn_layer_norm gave them
+ *   dx [rows][d], dweight, dbias [d]: NULL = not wanted */
+typedef struct DisnLayerNormGrad {
+  int32_t type, reserved; /* reserved = 0 */
+  int64_t rows, d;
+  const void* dy;
+  int64_t lddy;
+  const void* x;
+  int64_t ldx;
+  const float* mean;
+  const float* rstd;
+  const void* weight;
+  const void* residual;
+  int64_t ldr;
+  void* dx;
+  int64_t lddx;
+  void* dweight;
+  void* dbias;
+} DisnLayerNormGrad;
+int disn_layer_norm_backward_workspace(DisnCtx* ctx, const DisnLayerNormGrad* a, size_t* bytes);
+int disn_layer_norm_backward(DisnCtx* ctx, const DisnLayerNormGrad* a, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- marching cubes ---------------------------------------------------- */
 /* Slab description.  A whole grid is {nx,ny,nz, 0, nz, 0, nz}. */
 typedef struct DisnMcGrid {
