@@ -87,7 +87,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm(NormArgs a) {
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < E; ++i) s += x[i];   // places behind the row hold 0
-    const float mean = group_sum<G>(s, lds, 0) * inv;
+    const float mean = group_sum<G>(s, lds, 0) / (float)d;   // a division: the mean of equal values is that value
     s = 0.0f;
 #pragma unroll
     for (int p = 0; p < P; ++p)
