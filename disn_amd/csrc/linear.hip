@@ -12,6 +12,8 @@
 //   k_rows_* at most 16 rows times a large matrix: W streams past at memory speed
 #include "dense.h"
 
+#include <atomic>
+
 namespace {
 
 typedef __attribute__((ext_vector_type(16))) float floatx16;
@@ -21,6 +23,7 @@ typedef __attribute__((ext_vector_type(8))) short shortx8;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((address_space(3))) shortx4 lds_shortx4;
+typedef __attribute__((address_space(3))) char lds_char;
 
 // ---- activations ------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float activate(float z, int act) {
@@ -29,6 +32,23 @@ __device__ __forceinline__ float activate(float z, int act) {
     case DISN_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
     case DISN_ACT_SILU: return z / (1.0f + expf(-z));
     default: return z;
+  }
+}
+template <int N>
+__device__ __forceinline__ void activate_all(float (&z)[N], int act) {
+  switch (act) {   // one branch for all of them
+    case DISN_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) z[i] = activate(z[i], DISN_ACT_RELU);
+      break;
+    case DISN_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) z[i] = activate(z[i], DISN_ACT_GELU);
+      break;
+    case DISN_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) z[i] = activate(z[i], DISN_ACT_SILU);
+      break;
   }
 }
 // act'(z)
@@ -60,14 +80,14 @@ __device__ __forceinline__ void finish_one(const Epilogue& e, int64_t row, int c
   if (e.residual) y += (float)((const T*)e.residual)[row * e.ldr + col];
   ((T*)e.out)[row * e.ldo + col] = (T)y;
 }
-// n (>= 1) of Vec<T>::N values in a row
+// n (>= 1) of Vec<T>::N values in a row; the bias and the residual (anything where there is none) have been read before
 template <typename T>
-__device__ __forceinline__ void finish_vec(const Epilogue& e, int64_t row, int col, float (&z)[Vec<T>::N], int n) {
+__device__ __forceinline__ void finish_vec(const Epilogue& e, int64_t row, int col, float (&z)[Vec<T>::N], int n, const Vec<T>& bias,
+                                           const Vec<T>& residual) {
   constexpr int N = Vec<T>::N;
   if (e.bias) {
-    const Vec<T> b = load_vec((const T*)e.bias + col, n);
 #pragma unroll
-    for (int i = 0; i < N; ++i) z[i] += (float)b.v[i];
+    for (int i = 0; i < N; ++i) z[i] += (float)bias.v[i];
   }
   Vec<T> o;
   if (e.pre) {
@@ -75,16 +95,22 @@ __device__ __forceinline__ void finish_vec(const Epilogue& e, int64_t row, int c
     for (int i = 0; i < N; ++i) o.v[i] = (T)z[i];
     store_vec((T*)e.pre + row * e.ldp + col, o, n);
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i) z[i] = activate(z[i], e.act);
+  activate_all(z, e.act);
   if (e.residual) {
-    const Vec<T> r = load_vec((const T*)e.residual + row * e.ldr + col, n);
 #pragma unroll
-    for (int i = 0; i < N; ++i) z[i] += (float)r.v[i];
+    for (int i = 0; i < N; ++i) z[i] += (float)residual.v[i];
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) o.v[i] = (T)z[i];
   store_vec((T*)e.out + row * e.ldo + col, o, n);
+}
+template <typename T>
+__device__ __forceinline__ Vec<T> bias_vec(const Epilogue& e, int col, int n) {
+  return e.bias && n > 0 ? load_vec((const T*)e.bias + col, n) : Vec<T>{};
+}
+template <typename T>
+__device__ __forceinline__ Vec<T> residual_vec(const Epilogue& e, int64_t row, int col, int n) {
+  return e.residual && n > 0 ? load_vec((const T*)e.residual + row * e.ldr + col, n) : Vec<T>{};
 }
 
 // sums the partial products of a split r (0 of them: an empty sum) in order and finishes them
@@ -108,8 +134,93 @@ __global__ __launch_bounds__(256) void k_finish(const float* __restrict__ part, 
         for (int q = 0; q < 4; ++q) z[i + q] += v.v[q];
       }
     }
-    finish_vec<T>(e, row, col, z, n);
+    finish_vec<T>(e, row, col, z, n, bias_vec<T>(e, col, n), residual_vec<T>(e, row, col, n));
   }
+}
+
+// ---- tiles: what both kernels share ---------------------------------------------------------------------------------
+struct TileArgs {
+  const void *A, *B;
+  int64_t lda, ldb;
+  int M, N;
+  int64_t K, per;          // r values in all and per split (a multiple of KT)
+  int mt, nt, splits;
+  float* part;             // [splits][M][N], splits > 1
+  Epilogue e;
+};
+
+constexpr int tile_stride(int NB) { return NB * 32 + 4; }   // floats between the turned rows
+
+// The end of a tile: a wave's MB x NB sums (i from iw, j from jw on) become partial products or finished values.
+// Finishing goes through LDS (the stages' buffers, which the caller's waves have stopped reading once they meet here),
+// 32 rows at a time, so that a lane finishes 16 bytes of one row.
+// Lane's place in a 32 x 32 tile of C: j = l & 31, i = (g & 3) + 8 (g >> 2) + 4 (l >> 5).
+template <typename T, int MB, int NB, int WAVES>
+__device__ __forceinline__ void tile_end(const TileArgs& a, int split, int iw, int jw, const floatx16 (&acc)[MB][NB], float* lds) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, cj = lane & 31, ci = 4 * (lane >> 5);
+  if (a.splits > 1) {
+    float* part = a.part + (size_t)split * a.M * a.N;
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int g = 0; g < 16; ++g) {
+          const int i = iw + m * 32 + ci + (g & 3) + 8 * (g >> 2), j = jw + n * 32 + cj;
+          if (i < a.M && j < a.N) part[(size_t)i * a.N + j] = acc[m][n][g];
+        }
+    return;
+  }
+  // Memory operations of a wave end in order, so a wait for a load is a wait for the stores before it: the bias is read
+  // once, the next rows' residual before the present rows are stored.
+  constexpr int W = NB * 32, V = Vec<T>::N, STRIDE = tile_stride(NB), Q = 32 * W / V / 64;
+  const int r0 = lane / (W / V), c = lane % (W / V) * V, j = jw + c, n_j = a.N - j;
+  const Vec<T> bias = bias_vec<T>(a.e, j, n_j);
+  Vec<T> res[2][Q];
+  auto read_residual = [&](int m) {
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int i = iw + m * 32 + r0 + q * (64 / (W / V));
+      res[m & 1][q] = residual_vec<T>(a.e, i, j, i < a.M ? n_j : 0);
+    }
+  };
+  read_residual(0);
+  __syncthreads();
+  float* mine = lds + wave * (32 * STRIDE);
+#pragma unroll
+  for (int m = 0; m < MB; ++m) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int g = 0; g < 16; ++g) mine[(ci + (g & 3) + 8 * (g >> 2)) * STRIDE + n * 32 + cj] = acc[m][n][g];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    float z[Q][V];
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      __builtin_memcpy(z[q], __builtin_assume_aligned(mine + (r0 + q * (64 / (W / V))) * STRIDE + c, 16), sizeof z[q]);
+    if (m + 1 < MB) read_residual(m + 1);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int i = iw + m * 32 + r0 + q * (64 / (W / V));
+      if (i < a.M && n_j > 0) finish_vec<T>(a.e, i, j, z[q], n_j, bias, res[m & 1][q]);
+    }
+  }
+}
+
+// a workgroup's tile: the workgroups go to the 8 XCDs in turn; consecutive tiles share operands, so each XCD (own
+// L2) takes a run of them
+struct TilePlace {
+  int i0, j0, split;
+};
+__device__ __forceinline__ TilePlace tile_place(const TileArgs& a, int BM, int BN) {
+  const int total = a.mt * a.nt * a.splits, run = total >> 3, rest = total & 7, xcd = blockIdx.x & 7;
+  int id = (blockIdx.x >> 3) + xcd * run + (xcd < rest ? xcd : rest);
+  const int tn = id % a.nt;
+  id /= a.nt;
+  return {id % a.mt * BM, tn * BN, id / a.mt};
 }
 
 // ---- k_tile --------------------------------------------------------------------------------------------------------
@@ -235,16 +346,6 @@ struct Operand {
   }
 };
 
-struct TileArgs {
-  const void *A, *B;
-  int64_t lda, ldb;
-  int M, N;
-  int64_t K, per;          // r values in all and per split (a multiple of KT)
-  int mt, nt, splits;
-  float* part;             // [splits][M][N], splits > 1
-  Epilogue e;
-};
-
 template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void k_tile(TileArgs a) {
   constexpr int THREADS = WM * WN * 64, MB = BM / WM / 32, NB = BN / WN / 32, KT = Mma<T>::KT, P = Mma<T>::planes;
@@ -252,13 +353,8 @@ __global__ __launch_bounds__(WM * WN * 64) void k_tile(TileArgs a) {
   typedef Operand<T, B_ACROSS, BN, THREADS> OpB;
   constexpr int BUF = OpA::BYTES + OpB::BYTES;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  // Workgroups go to the 8 XCDs in turn; consecutive tiles share operands, so each XCD (own L2) takes a run of them.
-  const int total = a.mt * a.nt * a.splits, run = total >> 3, rest = total & 7, xcd = blockIdx.x & 7;
-  int id = (blockIdx.x >> 3) + xcd * run + (xcd < rest ? xcd : rest);
-  const int tn = id % a.nt;
-  id /= a.nt;
-  const int tm = id % a.mt, split = id / a.mt;
-  const int i0 = tm * BM, j0 = tn * BN;
+  const TilePlace at = tile_place(a, BM, BN);
+  const int i0 = at.i0, j0 = at.j0, split = at.split;
   const int64_t k0 = split * a.per;
   const int have = (int)(a.K - k0 < a.per ? a.K - k0 : a.per), stages = (have + KT - 1) / KT;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -323,7 +419,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_tile(TileArgs a) {
     }
   }
 
-  // lane's place in a 32 x 32 tile of C: j = l & 31, i = (g & 3) + 8 (g >> 2) + 4 (l >> 5)
+  static_assert(32 * tile_stride(NB) * 4 * WM * WN <= 2 * BUF, "the turned tiles fit into the stage buffers");
   const int cj = lane & 31, ci = 4 * (lane >> 5);
   if constexpr (P == 3) {
     bool bad = false;
@@ -358,43 +454,182 @@ __global__ __launch_bounds__(WM * WN * 64) void k_tile(TileArgs a) {
     }
   }
 
-  if (a.splits > 1) {
-    float* part = a.part + (size_t)split * a.M * a.N;
-#pragma unroll
-    for (int m = 0; m < MB; ++m)
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int g = 0; g < 16; ++g) {
-          const int i = i0 + wi + m * 32 + ci + (g & 3) + 8 * (g >> 2), j = j0 + wj + n * 32 + cj;
-          if (i < a.M && j < a.N) part[(size_t)i * a.N + j] = acc[m][n][g];
-        }
-    return;
+  tile_end<T, MB, NB, WM * WN>(a, split, i0 + wi, j0 + wj, acc, (float*)lds);
+}
+
+// ---- k_tile16 ------------------------------------------------------------------------------------------------------
+// bf16 and fp16.  A ring of four LDS stages of 32 r is filled by DMA (global_load_lds_dwordx4: no registers, no LDS
+// store instructions), so three stages, 96 KB a CU with 256-wide tiles, are on their way while one is multiplied.  Two
+// steps of 16 r a stage, and the fragments of a step are read while the step before is multiplied; the one barrier of a
+// stage lies between its two steps, when the second step's fragments are in registers: no wave waits for LDS behind it.
+//
+// A wave's DMA writes 1 KB of LDS in lane order, from any 16-byte pieces of memory.  Along r, LDS holds [i][32 r] (64
+// bytes), and the four pieces of a row are exchanged by (i >> 2) & 3: sixteen lanes of a fragment, sixteen rows, touch
+// all 64 banks.  Across r it holds [r][i], pieces exchanged by (r & 3) << 2: the four rows that 32 lanes read through
+// ds_read_b64_tr_b16, 64 bytes of each, lie on different banks.  Needs operands on 16-byte boundaries; others are copied first
+// (k_pack).  The last stage, where r is not a multiple of 32, goes through registers, with zeros behind it.
+constexpr int KT16 = 32, RING = 4;
+template <typename T, bool ACROSS, int ROWS, int WAVES, int BLOCKS>
+struct Operand16 {
+  static constexpr int BYTES = ROWS * KT16 * 2, PIECES = BYTES / 1024 / WAVES, PER_LINE = (ACROSS ? ROWS : KT16) / 8;
+  static_assert(PIECES * 1024 * WAVES == BYTES, "pieces");
+  const char* base;        // uniform: the stage to come
+  int64_t step;            // bytes between stages
+  unsigned off[PIECES];    // this lane's piece, relative to base
+  int left;
+
+  __device__ __forceinline__ static int line_of(int p) { return ((threadIdx.x >> 6) * PIECES + p) * (64 / PER_LINE) + (threadIdx.x & 63) / PER_LINE; }
+  __device__ __forceinline__ static int piece_of(int line) {
+    return ((threadIdx.x & 63) % PER_LINE) ^ (ACROSS ? (line & 3) << 2 : (line >> 2) & 3);
   }
-  // each wave turns its 32 rows at a time through LDS, so that a lane finishes 16 bytes of one row
-  constexpr int W = NB * 32, V = Vec<T>::N, STRIDE = W + 4;
-  static_assert(32 * STRIDE * 4 * WM * WN <= 2 * BUF, "the turned tiles fit into the stage buffers");
-  __syncthreads();
-  float* mine = (float*)lds + wave * (32 * STRIDE);
+  __device__ __forceinline__ void init(const void* p, int64_t ld, int i0, int n_i, int64_t k0) {
+    left = n_i - i0;
+    base = (const char*)p + (ACROSS ? k0 * ld + i0 : (int64_t)i0 * ld + k0) * 2;
+    step = (ACROSS ? KT16 * ld : KT16) * 2;
 #pragma unroll
-  for (int m = 0; m < MB; ++m) {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    for (int p = 0; p < PIECES; ++p) {
+      const int line = line_of(p), c = piece_of(line) * 8;
+      // outside the matrix: its last row, its first columns; they only reach sums nobody stores
+      off[p] = ACROSS ? (unsigned)(line * ld + (c < left ? c : 0)) * 2 : (unsigned)((line < left ? line : left - 1) * ld + c) * 2;
+    }
+  }
+  // the next stage into LDS at dst; have: how many r values exist from it on
+  __device__ __forceinline__ void fetch(char* dst, int have) {
+    dst += (threadIdx.x >> 6) * (PIECES * 1024);
+    if (have >= KT16) {
+      const unsigned m0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(lds_char*)dst);
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0 + p * 1024), "v"(off[p]), "s"(base) : "memory");
+    } else {
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) {
+        const int line = line_of(p), c = piece_of(line) * 8;
+        const T* src = (const T*)(base + off[p]);
+        Vec<T> v;
+        if (ACROSS)
+          v = load_vec(line < have ? src : (const T*)base, line < have ? (c < left ? left - c : left) : 0);
+        else
+          v = load_vec(c < have ? src : (const T*)base, have - c);
+        __builtin_memcpy(__builtin_assume_aligned(dst + p * 1024 + (threadIdx.x & 63) * 16, 16), &v, 16);
+      }
+    }
+    base += step;
+  }
+  // byte offsets of this lane's part of a wave's fragments, whose i values start at iw (a multiple of 32): along r one for
+  // each step of 16 r, across r one for each block of 32 i
+  static constexpr int OFFSETS = ACROSS ? BLOCKS : 2;
+  __device__ __forceinline__ static void lane_offsets(int iw, unsigned (&o)[OFFSETS]) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+#pragma unroll
+    for (int v = 0; v < OFFSETS; ++v) {
+      if (ACROSS) {
+        const int q = lane & 15, r = q >> 2;
+        const int piece = ((iw / 8 + v * 4) | ((lane & 16) >> 3) | ((q & 3) >> 1)) ^ (r << 2);
+        o[v] = (8 * h + r) * (ROWS * 2) + piece * 16 + (q & 1) * 8;
+      } else {
+        const int r = lane & 31;
+        o[v] = (iw + r) * 64 + (((2 * v + h) ^ ((r >> 2) & 3)) * 16);
+      }
+    }
+  }
+  // fragment of 32 i values of block `block`, 16 r values from 16 s
+  __device__ __forceinline__ static shortx8 fragment(const char* lds, const unsigned (&o)[OFFSETS], int block, int s) {
+    if constexpr (ACROSS) {
+      const char* p = lds + o[block] + s * (16 * ROWS * 2);
+      const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)(p));
+      const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)(p + 4 * ROWS * 2));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      return *(const shortx8*)(lds + o[s] + block * (32 * 64));
+    }
+  }
+};
+
+template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64) void k_tile16(TileArgs a) {
+  constexpr int WAVES = WM * WN, MB = BM / WM / 32, NB = BN / WN / 32;
+  typedef Operand16<T, A_ACROSS, BM, WAVES, MB> OpA;
+  typedef Operand16<T, B_ACROSS, BN, WAVES, NB> OpB;
+  constexpr int BUF = OpA::BYTES + OpB::BYTES, LOADS = OpA::PIECES + OpB::PIECES;
+  static_assert(32 * tile_stride(NB) * 4 * WAVES <= RING * BUF, "the turned tiles fit into the ring");
+  static_assert(LOADS == 4, "waits count four loads a stage");
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const TilePlace at = tile_place(a, BM, BN);
+  const int64_t k0 = at.split * a.per;
+  const int have = (int)(a.K - k0 < a.per ? a.K - k0 : a.per), stages = (have + KT16 - 1) / KT16, whole = have / KT16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WN * (MB * 32), wj = wave % WN * (NB * 32);
+
+  floatx16 acc[MB][NB];
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int g = 0; g < 16; ++g) mine[(ci + (g & 3) + 8 * (g >> 2)) * STRIDE + n * 32 + cj] = acc[m][n][g];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+      for (int g = 0; g < 16; ++g) acc[m][n][g] = 0.0f;
+  OpA A;
+  OpB B;
+  A.init(a.A, a.lda, at.i0, a.M, k0);
+  B.init(a.B, a.ldb, at.j0, a.N, k0);
+  unsigned oa[OpA::OFFSETS], ob[OpB::OFFSETS];
+  OpA::lane_offsets(wi, oa);
+  OpB::lane_offsets(wj, ob);
+  auto fetch = [&](int t) {
+    if (t >= stages) return;
+    char* dst = lds + (t & (RING - 1)) * BUF;
+    A.fetch(dst, have - t * KT16);
+    B.fetch(dst + OpA::BYTES, have - t * KT16);
+  };
+  shortx8 fa[2][MB], fb[2][NB];
+  auto read = [&](int t, int s) {
+    const char* p = lds + (t & (RING - 1)) * BUF;
 #pragma unroll
-    for (int q = 0; q < 32 * W / V / 64; ++q) {
-      const int t = lane + q * 64, r = t / (W / V), c = t % (W / V) * V;
-      const int i = i0 + wi + m * 32 + r, j = j0 + wj + c;
-      if (i >= a.M || j >= a.N) continue;
-      float z[V];
-      __builtin_memcpy(z, __builtin_assume_aligned(mine + r * STRIDE + c, 16), sizeof z);
-      finish_vec<T>(a.e, i, j, z, a.N - j);
+    for (int n = 0; n < NB; ++n) fb[s][n] = OpB::fragment(p + OpA::BYTES, ob, n, s);
+#pragma unroll
+    for (int m = 0; m < MB; ++m) fa[s][m] = OpA::fragment(p, oa, m, s);
+  };
+  auto multiply = [&](int s) {
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) acc[m][n] = mfma<T>(fa[s][m], fb[s][n], acc[m][n]);
+  };
+  // stage t has landed for everyone, and everyone has read what it wants of the stage before.  Stages up to t + 2 are
+  // under way, four loads of this wave each (the last, partial one has none).
+  auto meet = [&](int t) {
+    const int behind = min(t + 3, whole) - (t + 1);
+    if (behind >= 2) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    else if (behind == 1) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+  fetch(0);
+  fetch(1);
+  fetch(2);
+  meet(0);
+  fetch(3);
+  read(0, 0);
+  for (int t = 0; t < stages; ++t) {
+    read(t, 1);
+    multiply(0);
+    if (t + 1 < stages) {
+      meet(t + 1);
+      fetch(t + 4);
+      read(t + 1, 0);
     }
+    multiply(1);
+  }
+  tile_end<T, MB, NB, WAVES>(a, at.split, at.i0 + wi, at.j0 + wj, acc, (float*)lds);
+}
+
+// a copy of a 16-bit matrix on 16-byte boundaries
+template <typename T>
+__global__ __launch_bounds__(256) void k_pack(const T* __restrict__ src, int64_t lds_, T* __restrict__ dst, int64_t ldd, int64_t rows, int cols) {
+  const int64_t per = ldd / 8, total = rows * per;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+    const int64_t r = t / per;
+    const int c = (int)(t - r * per) * 8;
+    const Vec<T> v = load_vec(src + r * lds_ + c, cols - c);
+    store_vec(dst + r * ldd + c, v, 8);
   }
 }
 
@@ -721,17 +956,24 @@ struct Product {
 };
 struct Plan {
   Kind kind;
-  int tile;            // 128 or 256
+  int tile;                  // 128 or 256
   int splits;
   int64_t per;
-  size_t bytes;        // of partial sums
+  size_t pack_a, pack_b;     // bytes of copies on 16-byte boundaries (k_tile16), 0: none
+  size_t bytes;              // of workspace: the copies, then the partial sums
 };
+size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+// k_tile16 reads 16-byte pieces at 32-bit offsets from a tile's first value
+bool tile16_ready(const void* p, int64_t ld) { return dense_aligned(p, 16) && ld % 8 == 0 && ld <= 1 << 22; }
+size_t pack_bytes(int64_t rows, int64_t cols) { return align256((size_t)rows * ((cols + 7) / 8 * 8) * 2); }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-Plan plan(int type, bool a_across, bool b_across, int64_t M, int64_t N, int64_t K) {
-  Plan p{K_EMPTY, 0, 0, 0, 0};
+Plan plan(int type, const Product& q) {
+  Plan p{};
+  const bool a_across = q.a_across, b_across = q.b_across;
+  const int64_t M = q.M, N = q.N, K = q.K;
   if (M == 0 || N == 0 || K == 0) return p;
-  const int V = type == DISN_F32 ? 4 : 8, KT = type == DISN_F32 ? 16 : 64;
+  const int V = type == DISN_F32 ? 4 : 8, KT = type == DISN_F32 ? Mma<float>::KT : KT16;
   if (!a_across && M <= 16 && K * N >= (1 << 20)) {
     p.kind = K_ROWS;
     if (!b_across) return p;
@@ -751,11 +993,13 @@ Plan plan(int type, bool a_across, bool b_across, int64_t M, int64_t N, int64_t 
   p.tile = ceil_div(M, 256) * ceil_div(N, 256) >= 256 ? 256 : 128;
   const int64_t tiles = ceil_div(M, p.tile) * ceil_div(N, p.tile);
   int64_t want = tiles >= 256 ? 1 : 512 / tiles;
-  const int64_t most = ceil_div(K, 4 * KT);
+  const int64_t most = ceil_div(K, type == DISN_F32 ? 64 : 256);
   if (want > most) want = most;
   p.per = ceil_div(ceil_div(K, want), KT) * KT;
   p.splits = (int)ceil_div(K, p.per);
-  p.bytes = p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0;
+  if (type != DISN_F32 && !tile16_ready(q.A, q.lda)) p.pack_a = a_across ? pack_bytes(K, M) : pack_bytes(M, K);
+  if (type != DISN_F32 && !tile16_ready(q.B, q.ldb)) p.pack_b = b_across ? pack_bytes(K, N) : pack_bytes(N, K);
+  p.bytes = p.pack_a + p.pack_b + (p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0);
   return p;
 }
 
@@ -771,18 +1015,39 @@ int launch_finish(DisnCtx* ctx, const float* part, int nparts, int64_t M, int64_
 template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN>
 int launch_tile(DisnCtx* ctx, const TileArgs& a, hipStream_t stream) {
   constexpr int THREADS = WM * WN * 64;
-  constexpr int bytes = 2 * (Operand<T, A_ACROSS, BM, THREADS>::BYTES + Operand<T, B_ACROSS, BN, THREADS>::BYTES);
-  static_assert(bytes <= 160 * 1024, "LDS");
-  auto* kernel = k_tile<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN>;
-  DISN_HIP(ctx, hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  kernel<<<(unsigned)((int64_t)a.mt * a.nt * a.splits), THREADS, bytes, stream>>>(a);
-  DISN_HIP(ctx, hipGetLastError());
+  const void* kernel;
+  int bytes;
+  if constexpr (sizeof(T) == 4) {
+    kernel = (const void*)k_tile<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN>;
+    bytes = 2 * (Operand<T, A_ACROSS, BM, THREADS>::BYTES + Operand<T, B_ACROSS, BN, THREADS>::BYTES);
+  } else {
+    kernel = (const void*)k_tile16<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN>;
+    bytes = RING * (BM + BN) * KT16 * 2;
+  }
+  static std::atomic<uint64_t> ready{0};   // devices that allow this kernel its LDS
+  const uint64_t bit = 1ull << (ctx->device & 63);
+  if (!(ready.load() & bit)) {
+    DISN_HIP(ctx, hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    ready.fetch_or(bit);
+  }
+  TileArgs copy = a;
+  void* args[] = {&copy};
+  DISN_HIP(ctx, hipLaunchKernel(kernel, dim3((unsigned)((int64_t)a.mt * a.nt * a.splits)), dim3(THREADS), args, bytes, stream));
   return DISN_OK;
 }
 template <typename T, bool A_ACROSS, bool B_ACROSS>
 int launch_tile(DisnCtx* ctx, int tile, const TileArgs& a, hipStream_t stream) {
   return tile == 256 ? launch_tile<T, A_ACROSS, B_ACROSS, 256, 256, 2, 4>(ctx, a, stream)
                      : launch_tile<T, A_ACROSS, B_ACROSS, 128, 128, 2, 2>(ctx, a, stream);
+}
+// a copy of rows x cols values at dst, 16-byte boundaries; *p, *ld become it
+template <typename T>
+int launch_pack(DisnCtx* ctx, const void** p, int64_t* ld, int64_t rows, int64_t cols, char* dst, hipStream_t stream) {
+  const int64_t ldd = ceil_div(cols, 8) * 8, blocks = ceil_div(rows * ldd / 8, 256);
+  k_pack<T><<<(unsigned)(blocks < 8192 ? blocks : 8192), 256, 0, stream>>>((const T*)*p, *ld, (T*)dst, ldd, rows, (int)cols);
+  DISN_HIP(ctx, hipGetLastError());
+  *p = dst, *ld = ldd;
+  return DISN_OK;
 }
 
 template <typename T, int MR>
@@ -804,9 +1069,14 @@ SmallArgs small_args(const Product& q, const Plan&) {
 }
 int64_t small_blocks(const SmallArgs& s) { return (int64_t)s.mt * ceil_div(s.nt, SMALL_WAVES / s.ks); }
 
-// one product by its plan; part: plan.bytes of workspace
+// one product by its plan; ws: plan.bytes of workspace
 template <typename T>
-int run_product(DisnCtx* ctx, const Product& q, const Plan& p, float* part, hipStream_t stream) {
+int run_product(DisnCtx* ctx, Product q, const Plan& p, char* ws, hipStream_t stream) {
+  float* part = (float*)(ws + p.pack_a + p.pack_b);
+  if constexpr (sizeof(T) == 2) {
+    if (p.pack_a) DISN_TRY(launch_pack<T>(ctx, &q.A, &q.lda, q.a_across ? q.K : q.M, q.a_across ? q.M : q.K, ws, stream));
+    if (p.pack_b) DISN_TRY(launch_pack<T>(ctx, &q.B, &q.ldb, q.b_across ? q.K : q.N, q.b_across ? q.N : q.K, ws + p.pack_a, stream));
+  }
   if (q.M == 0 || q.N == 0) return DISN_OK;
   if (p.kind == K_EMPTY) return launch_finish<T>(ctx, nullptr, 0, q.M, q.N, q.e, stream);
   if (p.kind == K_SMALL) {
@@ -890,16 +1160,25 @@ struct GradPlan {
   int gate_lanes, gate_groups;
   size_t off_sums, off_part, bytes;   // workspace: dz, partial column sums, partial products
 };
-size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+// the two products on dz as it lies at (dz, ldz)
+void grad_products(const DisnLinearGrad* a, const void* dz, int64_t ldz, Product* dx, Product* dw) {
+  *dx = {dz, a->w, ldz, a->ldw, false, a->w_nk != 0, a->m, a->k, a->n, {nullptr, nullptr, nullptr, a->dx, 0, 0, a->lddx, DISN_ACT_NONE}};
+  *dw = {a->x, dz, a->ldx, ldz, true, true, a->k, a->n, a->m, {nullptr, nullptr, nullptr, a->dw, 0, 0, a->lddw, DISN_ACT_NONE}};
+  if (a->w_nk) *dw = {dz, a->x, ldz, a->ldx, true, true, a->n, a->k, a->m, dw->e};
+}
 GradPlan plan_backward(const DisnLinearGrad* a) {
   GradPlan g{};
   const size_t s = dense_type_size(a->type);
-  if (a->dx) g.dx = plan(a->type, false, a->w_nk != 0, a->m, a->k, a->n);
-  if (a->dw) g.dw = a->w_nk ? plan(a->type, true, true, a->n, a->k, a->m) : plan(a->type, true, true, a->k, a->n, a->m);
+  Product dx, dw;
+  g.ldz = ceil_div(a->n, 8) * 8;
+  // dz of an activation will lie in the workspace, at an address like 256
+  if (a->act != DISN_ACT_NONE) grad_products(a, (const void*)256, g.ldz, &dx, &dw);
+  else grad_products(a, a->dy, a->lddy, &dx, &dw);
+  if (a->dx) g.dx = plan(a->type, dx);
+  if (a->dw) g.dw = plan(a->type, dw);
   g.small = a->dw && g.dw.kind == K_SMALL && (!a->dx || g.dx.kind == K_SMALL);
   if (g.small) return g;
   const int V = (int)(16 / s);
-  g.ldz = ceil_div(a->n, V) * V;
   g.gate_lanes = 1;
   while (g.gate_lanes < 64 && g.gate_lanes * V < a->n) g.gate_lanes *= 2;
   g.gate_groups = (int)ceil_div(a->n, g.gate_lanes * V);
@@ -941,12 +1220,11 @@ int run_backward(DisnCtx* ctx, const DisnLinearGrad* a, const GradPlan& g, char*
     }
     if (write) dz = ws, ldz = g.ldz;
   }
-  Product dx{dz, a->w, ldz, a->ldw, false, a->w_nk != 0, a->m, a->k, a->n, {nullptr, nullptr, nullptr, a->dx, 0, 0, a->lddx, DISN_ACT_NONE}};
-  Product dw{a->x, dz, a->ldx, ldz, true, true, a->k, a->n, a->m, {nullptr, nullptr, nullptr, a->dw, 0, 0, a->lddw, DISN_ACT_NONE}};
-  if (a->w_nk) dw = {dz, a->x, ldz, a->ldx, true, true, a->n, a->k, a->m, dw.e};
+  Product dx, dw;
+  grad_products(a, dz, ldz, &dx, &dw);
   if (!g.small) {
-    if (a->dx) DISN_TRY(run_product<T>(ctx, dx, g.dx, (float*)(ws + g.off_part), stream));
-    if (a->dw) DISN_TRY(run_product<T>(ctx, dw, g.dw, (float*)(ws + g.off_part), stream));
+    if (a->dx) DISN_TRY(run_product<T>(ctx, dx, g.dx, ws + g.off_part, stream));
+    if (a->dw) DISN_TRY(run_product<T>(ctx, dw, g.dw, ws + g.off_part, stream));
     return DISN_OK;
   }
   SmallArgs sx = small_args(dx, g.dx), sw = small_args(dw, g.dw);
@@ -970,19 +1248,19 @@ extern "C" int disn_linear_workspace(DisnCtx* ctx, const DisnLinear* a, size_t* 
   if (!ctx) return DISN_E_ARG;
   if (!bytes) return disn_fail(ctx, DISN_E_ARG, "disn_linear_workspace: null result");
   DISN_TRY(check_linear(ctx, a));
-  *bytes = plan(a->type, false, a->w_nk == 0, a->m, a->n, a->k).bytes;
+  *bytes = plan(a->type, forward_product(a)).bytes;
   return DISN_OK;
 }
 
 extern "C" int disn_linear(DisnCtx* ctx, const DisnLinear* a, void* workspace, size_t workspace_bytes, void* stream) {
   if (!ctx) return DISN_E_ARG;
   DISN_TRY(check_linear(ctx, a));
-  const Plan p = plan(a->type, false, a->w_nk == 0, a->m, a->n, a->k);
+  const Plan p = plan(a->type, forward_product(a));
   if (p.bytes && (!workspace || !dense_aligned(workspace, 16) || workspace_bytes < p.bytes))
     return disn_fail(ctx, DISN_E_ARG, "disn_linear: needs %zu bytes of 16-byte aligned workspace", p.bytes);
   DISN_HIP(ctx, hipSetDevice(ctx->device));
   return dense_dispatch(a->type, [&](auto t) {
-    return run_product<decltype(t)>(ctx, forward_product(a), p, (float*)workspace, (hipStream_t)stream);
+    return run_product<decltype(t)>(ctx, forward_product(a), p, (char*)workspace, (hipStream_t)stream);
   });
 }
 
