@@ -8,7 +8,6 @@ Reference counterparts:
   Context.marching_cubes <- create_obj / computeMarchingCubes (demo/demo.py:355-369)
 torch is used only for device memory and streams.
 """
-import contextlib
 import ctypes
 
 import numpy as np
@@ -226,10 +225,11 @@ class Context:
     # Tensors of a call: on the context's device, one type of float32 / bfloat16 / float16, rows along the last
     # dimension.  Rows may lie any distance apart (slices, expanded rows); another order is copied first.  The calls run
     # on the current stream, can be captured into graphs, and record no autograd history.
+    # A small call takes the GPU about 4 us, so the wrapper's own time counts: cheap checks, one struct, no copies where none
+    # are needed.
     def _tensor(self, t, what, dtype):
-        if not (isinstance(t, torch.Tensor) and t.device == self.device and t.dtype == dtype and t.layout == torch.strided):
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != self.device or t.layout is not torch.strided:
             raise DisnError("%s must be a %s tensor on %s" % (what, dtype, self.device))
-        return t
 
     def _rows(self, t, what, dtype, shape, copy=True):
         """a [..., c] tensor as a matrix -> (tensor, (address, rows, c, row distance, value size))"""
@@ -254,15 +254,20 @@ class Context:
         return t, (t.data_ptr(), n, c, c if n <= 1 else ld, t.element_size())
 
     def _vec(self, t, what, dtype, n):
+        """a vector of n values or None -> (tensor, address)"""
         if t is None:
-            return None
-        if self._tensor(t, what, dtype).shape != (n,):
+            return None, None
+        self._tensor(t, what, dtype)
+        if t.dim() != 1 or t.numel() != n:
             raise DisnError("%s has shape %s, expected (%d,)" % (what, tuple(t.shape), n))
-        return t.contiguous()
+        if not t.is_contiguous():
+            t = t.contiguous()
+        return t, t.data_ptr()
 
     def _weight(self, w, what, dtype):
         """[k][n] weights in either order of memory -> (tensor, w_nk, address, row distance)"""
-        if self._tensor(w, what, dtype).dim() != 2:
+        self._tensor(w, what, dtype)
+        if w.dim() != 2:
             raise DisnError("%s must be a [k, n] matrix" % what)
         k, n = w.shape
         s0, s1 = w.stride()
@@ -273,60 +278,65 @@ class Context:
         w = w.contiguous()
         return w, 0, w.data_ptr(), n
 
-    def _on_device(self):
-        """the context's device as the current one, as a context manager (free where it is current already)"""
-        return contextlib.nullcontext() if torch.cuda.current_device() == self.device.index else torch.cuda.device(self.device)
+    def _elsewhere(self):
+        """whether another device than the context's is the current one"""
+        return torch.cuda.current_device() != self.device.index
 
-    def _workspace(self, query, args, what):
-        n = ctypes.c_size_t()
-        self._check(query(self._h, ctypes.byref(args), ctypes.byref(n)), what)
-        return torch.empty(n.value, dtype=torch.uint8, device=self.device) if n.value else None
-
-    def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
+    def _run(self, query, call, name, args, like):
+        """a call with the workspace it asks for, on the current stream of the context's device"""
+        ws, n = None, ctypes.c_size_t()
+        ref = ctypes.byref(args)
+        if query is not None:
+            rc = query(self._h, ref, ctypes.byref(n))
+            if rc:
+                self._check(rc, name)
+            if n.value:
+                ws = like.new_empty(n.value, dtype=torch.uint8)
+        stream = torch._C._cuda_getCurrentRawStream(self.device.index)   # current_stream().cuda_stream without the object
+        rc = call(self._h, ref, stream) if query is None else call(self._h, ref, ws.data_ptr() if ws is not None else None, n.value, stream)
+        if rc:
+            self._check(rc, name)
 
     @staticmethod
     def _type(t, what):
-        if not isinstance(t, torch.Tensor) or t.dtype not in TYPES:
-            raise DisnError("%s must be a float32, bfloat16 or float16 tensor" % what)
+        if not isinstance(t, torch.Tensor) or t.dtype not in TYPES or t.dim() < 1:
+            raise DisnError("%s must be a float32, bfloat16 or float16 tensor of one dimension at least" % what)
         return t.dtype
 
     def linear(self, x, w, bias=None, residual=None, act="none", want_pre=False, out=None):
         """act(x @ w + bias) + residual (disn_linear).  x: [..., k]; w: [k, n] by rows, or the .t() of an [n, k] matrix;
         bias: [n]; residual: [..., n]; act: none, relu, gelu (erf), silu.  want_pre: -> (y, x @ w + bias), the second for
         linear_backward.  out: a tensor for y, which may be the residual itself but overlaps no other argument."""
+        if self._elsewhere():
+            with torch.cuda.device(self.device):
+                return self.linear(x, w, bias, residual, act, want_pre, out)
         dtype = self._type(x, "linear: x")
         if act not in ACTS:
             raise DisnError("linear: unknown act %r (have %s)" % (act, ", ".join(ACTS)))
-        if x.dim() < 1:
-            raise DisnError("linear: x must be [..., k]")
-        with self._on_device():
-            w, w_nk, wp, ldw = self._weight(w, "linear: w", dtype)
-            k, n = w.shape
-            shape = x.shape[:-1] + (n,)
-            x, xm = self._rows(x, "linear: x", dtype, x.shape[:-1] + (k,))
-            m = x.numel() // k if k else shape[:-1].numel()
-            bias = self._vec(bias, "linear: bias", dtype, n)
-            rm = (None, 0, 0, 0)
-            if residual is not None:
-                residual, rm = self._rows(residual, "linear: residual", dtype, shape)
-            if out is None:
-                y = torch.empty(shape, dtype=dtype, device=self.device)
-                ym = (y.data_ptr(), m, n, n)
-            else:
-                y, ym = self._rows(out, "linear: out", dtype, shape, copy=False)
-                size = xm[4]
-                wm = (wp, n, k, ldw, size) if w_nk else (wp, k, n, ldw, size)
-                if (_meet(ym, xm) or _meet(ym, wm) or (bias is not None and _meet(ym, (bias.data_ptr(), 1, n, n, size))) or
-                        (rm[0] is not None and _meet(ym, rm) and (ym[0], ym[3]) != (rm[0], rm[3]))):
-                    raise DisnError("linear: out overlaps another argument")
-            pre = torch.empty(shape, dtype=dtype, device=self.device) if want_pre else None
-            a = _lib.DisnLinear(TYPES[dtype], ACTS[act], w_nk, 0, m, n, k, xm[0], xm[3], wp, ldw,
-                                None if bias is None else bias.data_ptr(), rm[0], rm[3], ym[0], ym[3],
-                                pre.data_ptr() if want_pre else None, n)
-            ws = self._workspace(self.lib.disn_linear_workspace, a, "disn_linear_workspace")
-            self._check(self.lib.disn_linear(self._h, ctypes.byref(a), None if ws is None else ws.data_ptr(),
-                                             0 if ws is None else ws.numel(), self._stream()), "disn_linear")
+        w, w_nk, wp, ldw = self._weight(w, "linear: w", dtype)
+        k, n = w.shape
+        lead = x.shape[:-1]
+        shape = lead + (n,)
+        x, xm = self._rows(x, "linear: x", dtype, lead + (k,))
+        m = xm[1] if k else lead.numel()
+        bias, bp = self._vec(bias, "linear: bias", dtype, n)
+        rm = (None, 0, 0, 0)
+        if residual is not None:
+            residual, rm = self._rows(residual, "linear: residual", dtype, shape)
+        if out is None:
+            y = x.new_empty(shape)
+            yp, ldy = y.data_ptr(), n
+        else:
+            y, ym = self._rows(out, "linear: out", dtype, shape, copy=False)
+            yp, ldy, size = ym[0], ym[3], xm[4]
+            wm = (wp, n, k, ldw, size) if w_nk else (wp, k, n, ldw, size)
+            if (_meet(ym, xm) or _meet(ym, wm) or (bp is not None and _meet(ym, (bp, 1, n, n, size))) or
+                    (rm[0] is not None and _meet(ym, rm) and (yp, ldy) != (rm[0], rm[3]))):
+                raise DisnError("linear: out overlaps another argument")
+        pre = x.new_empty(shape) if want_pre else None
+        a = _lib.DisnLinear(TYPES[dtype], ACTS[act], w_nk, 0, m, n, k, xm[0], xm[3], wp, ldw, bp, rm[0], rm[3], yp, ldy,
+                            pre.data_ptr() if want_pre else None, n)
+        self._run(self.lib.disn_linear_workspace, self.lib.disn_linear, "disn_linear", a, x)
         return (y, pre) if want_pre else y
 
     def linear_backward(self, dy, x, w, pre=None, act="none", want_dx=True, want_dw=True, want_db=True):
@@ -334,96 +344,108 @@ class Context:
         x, w as in linear (w may be None without dx, x without dw); pre: linear's second result, not with act
         "none"; for relu without a residual y does as well.  dw lies in memory as w does.  The gradient of the
         residual is dy."""
+        if self._elsewhere():
+            with torch.cuda.device(self.device):
+                return self.linear_backward(dy, x, w, pre, act, want_dx, want_dw, want_db)
         dtype = self._type(dy, "linear_backward: dy")
         if act not in ACTS:
             raise DisnError("linear_backward: unknown act %r (have %s)" % (act, ", ".join(ACTS)))
         if (pre is None) != (act == "none"):
             raise DisnError("linear_backward: pre belongs to an activation (act %r)" % act)
-        if dy.dim() < 1 or (w is None and (want_dx or x is None) and (want_dx or want_dw)) or (x is None and want_dw):
-            raise DisnError("linear_backward: dx needs w, dw needs x, dy must be [..., n]")
-        with self._on_device():
-            n = dy.shape[-1]
-            lead = dy.shape[:-1]
-            m = lead.numel()
-            w_nk, wp, ldw, k = 0, None, 0, 0
-            if w is not None:
-                w, w_nk, wp, ldw = self._weight(w, "linear_backward: w", dtype)
-                k = w.shape[0]
-                if w.shape[1] != n:
-                    raise DisnError("linear_backward: w has shape %s, dy %s" % (tuple(w.shape), tuple(dy.shape)))
-            elif x is not None:
-                k = x.shape[-1]
-            dy, dm = self._rows(dy, "linear_backward: dy", dtype, dy.shape)
-            xm = pm = (None, 0, 0, 0)
-            if x is not None and want_dw:
-                x, xm = self._rows(x, "linear_backward: x", dtype, lead + (k,))
-            if pre is not None:
-                pre, pm = self._rows(pre, "linear_backward: pre", dtype, dy.shape)
-            dx = torch.empty(lead + (k,), dtype=dtype, device=self.device) if want_dx else None
-            dw = torch.empty((n, k) if w_nk else (k, n), dtype=dtype, device=self.device) if want_dw else None
-            db = torch.empty(n, dtype=dtype, device=self.device) if want_db else None
-            a = _lib.DisnLinearGrad(TYPES[dtype], ACTS[act], w_nk, 0, m, n, k, dm[0], dm[3], xm[0], xm[3], wp, ldw, pm[0], pm[3],
-                                    dx.data_ptr() if want_dx else None, k, dw.data_ptr() if want_dw else None, k if w_nk else n,
-                                    db.data_ptr() if want_db else None)
-            ws = self._workspace(self.lib.disn_linear_backward_workspace, a, "disn_linear_backward_workspace")
-            self._check(self.lib.disn_linear_backward(self._h, ctypes.byref(a), None if ws is None else ws.data_ptr(),
-                                                      0 if ws is None else ws.numel(), self._stream()), "disn_linear_backward")
+        if (w is None and want_dx) or (x is None and want_dw):
+            raise DisnError("linear_backward: dx needs w, dw needs x")
+        lead, n = dy.shape[:-1], dy.shape[-1]
+        w_nk, wp, ldw, k = 0, None, 0, 0
+        if w is not None:
+            w, w_nk, wp, ldw = self._weight(w, "linear_backward: w", dtype)
+            k = w.shape[0]
+            if w.shape[1] != n:
+                raise DisnError("linear_backward: w has shape %s, dy %s" % (tuple(w.shape), tuple(dy.shape)))
+        elif x is not None:
+            k = x.shape[-1]
+        dy, dm = self._rows(dy, "linear_backward: dy", dtype, dy.shape)
+        xm = pm = (None, 0, 0, 0)
+        if x is not None:
+            x, xm = self._rows(x, "linear_backward: x", dtype, lead + (k,))
+        if pre is not None:
+            pre, pm = self._rows(pre, "linear_backward: pre", dtype, dy.shape)
+        dx = dw = db = xp = dwp = dbp = None
+        if want_dx:
+            dx = dy.new_empty(lead + (k,))
+            xp = dx.data_ptr()
+        if want_dw:
+            dw = dy.new_empty((n, k) if w_nk else (k, n))
+            dwp = dw.data_ptr()
+        if want_db:
+            db = dy.new_empty(n)
+            dbp = db.data_ptr()
+        a = _lib.DisnLinearGrad(TYPES[dtype], ACTS[act], w_nk, 0, dm[1] if n else lead.numel(), n, k, dm[0], dm[3], xm[0], xm[3], wp, ldw,
+                                pm[0], pm[3], xp, k, dwp, k if w_nk else n, dbp)
+        self._run(self.lib.disn_linear_backward_workspace, self.lib.disn_linear_backward, "disn_linear_backward", a, dy)
         return dx, dw.t() if want_dw and w_nk else dw, db
 
     def layer_norm(self, x, weight=None, bias=None, eps=1e-5, want_stats=False, out=None):
         """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension (disn_layer_norm), which holds 1 to 8192
         values.  weight, bias: [d] or None (1, 0).  want_stats: -> (y, mean, rstd), the last two float32 [...], for
         layer_norm_backward.  out: a tensor for y that overlaps no argument."""
+        if self._elsewhere():
+            with torch.cuda.device(self.device):
+                return self.layer_norm(x, weight, bias, eps, want_stats, out)
         dtype = self._type(x, "layer_norm: x")
-        if x.dim() < 1:
-            raise DisnError("layer_norm: x must be [..., d]")
-        with self._on_device():
-            shape = x.shape
-            d, rows = shape[-1], shape[:-1].numel()
-            x, xm = self._rows(x, "layer_norm: x", dtype, shape)
-            weight, bias = self._vec(weight, "layer_norm: weight", dtype, d), self._vec(bias, "layer_norm: bias", dtype, d)
-            if out is None:
-                y = torch.empty(shape, dtype=dtype, device=self.device)
-                ym = (y.data_ptr(), rows, d, d)
-            else:
-                y, ym = self._rows(out, "layer_norm: out", dtype, shape, copy=False)
-                if _meet(ym, xm) or any(_meet(ym, (v.data_ptr(), 1, d, d, xm[4])) for v in (weight, bias) if v is not None):
-                    raise DisnError("layer_norm: out overlaps another argument")
-            mean, rstd = (torch.empty(shape[:-1], dtype=torch.float32, device=self.device) if want_stats else None for _ in (0, 1))
-            a = _lib.DisnLayerNorm(TYPES[dtype], 0, rows, d, xm[0], xm[3], None if weight is None else weight.data_ptr(),
-                                   None if bias is None else bias.data_ptr(), eps, ym[0], ym[3],
-                                   mean.data_ptr() if want_stats else None, rstd.data_ptr() if want_stats else None)
-            self._check(self.lib.disn_layer_norm(self._h, ctypes.byref(a), self._stream()), "disn_layer_norm")
+        shape = x.shape
+        lead, d = shape[:-1], shape[-1]
+        x, xm = self._rows(x, "layer_norm: x", dtype, shape)
+        weight, wp = self._vec(weight, "layer_norm: weight", dtype, d)
+        bias, bp = self._vec(bias, "layer_norm: bias", dtype, d)
+        if out is None:
+            y = x.new_empty(shape)
+            yp, ldy = y.data_ptr(), d
+        else:
+            y, ym = self._rows(out, "layer_norm: out", dtype, shape, copy=False)
+            yp, ldy = ym[0], ym[3]
+            if _meet(ym, xm) or any(_meet(ym, (v, 1, d, d, xm[4])) for v in (wp, bp) if v is not None):
+                raise DisnError("layer_norm: out overlaps another argument")
+        mean = rstd = mp = rp = None
+        if want_stats:
+            mean, rstd = x.new_empty(lead, dtype=torch.float32), x.new_empty(lead, dtype=torch.float32)
+            mp, rp = mean.data_ptr(), rstd.data_ptr()
+        a = _lib.DisnLayerNorm(TYPES[dtype], 0, xm[1], d, xm[0], xm[3], wp, bp, eps, yp, ldy, mp, rp)
+        self._run(None, self.lib.disn_layer_norm, "disn_layer_norm", a, x)
         return (y, mean, rstd) if want_stats else y
 
     def layer_norm_backward(self, dy, x, mean, rstd, weight=None, residual=None, want_dx=True, want_dweight=True, want_dbias=True):
         """Gradients of layer_norm (disn_layer_norm_backward) -> (dx, dweight, dbias), None for the ones not wanted.
         mean, rstd: layer_norm's; residual: [..., d], the gradient that reaches x past the norm, added to dx."""
+        if self._elsewhere():
+            with torch.cuda.device(self.device):
+                return self.layer_norm_backward(dy, x, mean, rstd, weight, residual, want_dx, want_dweight, want_dbias)
         dtype = self._type(dy, "layer_norm_backward: dy")
-        if dy.dim() < 1:
-            raise DisnError("layer_norm_backward: dy must be [..., d]")
-        with self._on_device():
-            shape = dy.shape
-            d, rows = shape[-1], shape[:-1].numel()
-            dy, dm = self._rows(dy, "layer_norm_backward: dy", dtype, shape)
-            x, xm = self._rows(x, "layer_norm_backward: x", dtype, shape)
-            for t, what in ((mean, "mean"), (rstd, "rstd")):
-                if self._tensor(t, "layer_norm_backward: " + what, torch.float32).shape != shape[:-1]:
-                    raise DisnError("layer_norm_backward: %s has shape %s, expected %s" % (what, tuple(t.shape), tuple(shape[:-1])))
-            mean, rstd = mean.contiguous(), rstd.contiguous()
-            weight = self._vec(weight, "layer_norm_backward: weight", dtype, d)
-            rm = (None, 0, 0, 0)
-            if residual is not None:
-                residual, rm = self._rows(residual, "layer_norm_backward: residual", dtype, shape)
-            dx = torch.empty(shape, dtype=dtype, device=self.device) if want_dx else None
-            dweight, dbias = (torch.empty(d, dtype=dtype, device=self.device) if v else None for v in (want_dweight, want_dbias))
-            a = _lib.DisnLayerNormGrad(TYPES[dtype], 0, rows, d, dm[0], dm[3], xm[0], xm[3], mean.data_ptr(), rstd.data_ptr(),
-                                       None if weight is None else weight.data_ptr(), rm[0], rm[3],
-                                       dx.data_ptr() if want_dx else None, d, dweight.data_ptr() if want_dweight else None,
-                                       dbias.data_ptr() if want_dbias else None)
-            ws = self._workspace(self.lib.disn_layer_norm_backward_workspace, a, "disn_layer_norm_backward_workspace")
-            self._check(self.lib.disn_layer_norm_backward(self._h, ctypes.byref(a), None if ws is None else ws.data_ptr(),
-                                                          0 if ws is None else ws.numel(), self._stream()), "disn_layer_norm_backward")
+        shape = dy.shape
+        lead, d = shape[:-1], shape[-1]
+        dy, dm = self._rows(dy, "layer_norm_backward: dy", dtype, shape)
+        x, xm = self._rows(x, "layer_norm_backward: x", dtype, shape)
+        self._tensor(mean, "layer_norm_backward: mean", torch.float32)
+        self._tensor(rstd, "layer_norm_backward: rstd", torch.float32)
+        if mean.shape != lead or rstd.shape != lead:
+            raise DisnError("layer_norm_backward: mean has shape %s, rstd %s, expected %s" % (tuple(mean.shape), tuple(rstd.shape), tuple(lead)))
+        mean, rstd = mean.contiguous(), rstd.contiguous()
+        weight, wp = self._vec(weight, "layer_norm_backward: weight", dtype, d)
+        rm = (None, 0, 0, 0)
+        if residual is not None:
+            residual, rm = self._rows(residual, "layer_norm_backward: residual", dtype, shape)
+        dx = dweight = dbias = xp = dwp = dbp = None
+        if want_dx:
+            dx = dy.new_empty(shape)
+            xp = dx.data_ptr()
+        if want_dweight:
+            dweight = dy.new_empty(d)
+            dwp = dweight.data_ptr()
+        if want_dbias:
+            dbias = dy.new_empty(d)
+            dbp = dbias.data_ptr()
+        a = _lib.DisnLayerNormGrad(TYPES[dtype], 0, dm[1], d, dm[0], dm[3], xm[0], xm[3], mean.data_ptr(), rstd.data_ptr(), wp, rm[0], rm[3],
+                                   xp, d, dwp, dbp)
+        self._run(self.lib.disn_layer_norm_backward_workspace, self.lib.disn_layer_norm_backward, "disn_layer_norm_backward", a, dy)
         return dx, dweight, dbias
 
     # ---- marching cubes ---------------------------------------------------

@@ -1,7 +1,5 @@
 """Dense layer and layer norm: what the wrapper makes of tensors and what it refuses, before any call into the library
 (no GPU: a context that was never opened, on the CPU)."""
-import contextlib
-
 import pytest
 import torch
 
@@ -12,8 +10,9 @@ from disn_amd import api
 def ctx(monkeypatch):
     c = api.Context.__new__(api.Context)
     c.device = torch.device("cpu")
-    monkeypatch.setattr(api.Context, "_on_device", lambda self: contextlib.nullcontext())
-    monkeypatch.setattr(api.Context, "_workspace", lambda *a: pytest.fail("the call should have been refused"))
+    c.lib = type("NoLibrary", (), {"__getattr__": lambda self, name: name})()
+    monkeypatch.setattr(api.Context, "_elsewhere", lambda self: False)
+    monkeypatch.setattr(api.Context, "_run", lambda *a: pytest.fail("the call should have been refused"))
     return c
 
 
@@ -67,7 +66,7 @@ def test_meet():
     (lambda c, x, w: c.linear(x, w.half()), "must be a torch.float32"),
     (lambda c, x, w: c.linear(x, w[0]), r"\[k, n\]"),
     (lambda c, x, w: c.linear(x, w[:5]), "expected"),
-    (lambda c, x, w: c.linear(x[0, 0], w), r"\[\.\.\., k\]"),
+    (lambda c, x, w: c.linear(x[0, 0], w), "one dimension"),
     (lambda c, x, w: c.linear(x, w, bias=torch.zeros(4)), "bias has shape"),
     (lambda c, x, w: c.linear(x, w, bias=torch.zeros(1, 6)), "bias has shape"),
     (lambda c, x, w: c.linear(x, w, residual=torch.zeros(6)), "residual has shape"),
