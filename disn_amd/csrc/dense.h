@@ -20,23 +20,52 @@ __device__ __forceinline__ Vec<T> load_vec(const T* p) {
   __builtin_memcpy(&r, p, 16);
   return r;
 }
-// the first n (<= N) values at p, zeros behind them; nothing beyond p[n - 1] is read
+// The first n values at p (n >= N: all, n <= 0: none), zeros behind them; nothing outside the row is read.  before: how
+// many values of the row lie in front of p; with N - n of them the piece is read from so much further in front and shifted.
+// (No sequence of single loads beside the wide one: hipcc merges the two into three narrow loads for every lane.)
 template <typename T>
-__device__ __forceinline__ Vec<T> load_vec(const T* p, int n) {
-  if (n >= Vec<T>::N) return load_vec(p);
-  Vec<T> r;
-#pragma unroll
-  for (int i = 0; i < Vec<T>::N; ++i) r.v[i] = i < n ? p[i] : (T)0.0f;
-  return r;
+__device__ __forceinline__ Vec<T> load_vec(const T* p, int n, int64_t before) {
+  constexpr int N = Vec<T>::N;
+  if (n >= N) return load_vec(p);
+  const int back = N - n;
+  uint64_t w[2] = {0, 0};
+  if (n > 0) {
+    if (back <= before) {
+      __builtin_memcpy(w, p - back, 16);
+      const int s = back * (8 * (int)sizeof(T));
+      if (s >= 64) {
+        w[0] = w[1] >> (s - 64);
+        w[1] = 0;
+      } else {
+        w[0] = (w[0] >> s) | ((w[1] << 1) << (63 - s));
+        w[1] >>= s;
+      }
+    } else {   // a row of fewer than N values
+#pragma unroll 1
+      for (int i = n - 1; i >= 0; --i) {
+        uint64_t bits = 0;
+        __builtin_memcpy(&bits, p + i, sizeof(T));
+        w[1] = (w[1] << (8 * sizeof(T))) | (w[0] >> (64 - 8 * sizeof(T)));
+        w[0] = (w[0] << (8 * sizeof(T))) | bits;
+      }
+    }
+  }
+  return __builtin_bit_cast(Vec<T>, w);
 }
+// the first n (n >= N: all) values to p
 template <typename T>
 __device__ __forceinline__ void store_vec(T* p, const Vec<T>& r, int n) {
   if (n >= Vec<T>::N) {
     __builtin_memcpy(p, &r, 16);
   } else {
-#pragma unroll
-    for (int i = 0; i < Vec<T>::N; ++i)
-      if (i < n) p[i] = r.v[i];
+    uint64_t w[2];
+    __builtin_memcpy(w, &r, 16);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      __builtin_memcpy(p + i, w, sizeof(T));
+      w[0] = (w[0] >> (8 * sizeof(T))) | (w[1] << (64 - 8 * sizeof(T)));
+      w[1] >>= 8 * sizeof(T);
+    }
   }
 }
 

@@ -26,11 +26,32 @@ typedef __attribute__((address_space(3))) shortx4 lds_shortx4;
 typedef __attribute__((address_space(3))) char lds_char;
 
 // ---- activations ------------------------------------------------------------------------------------------------
+// The normal distribution's upper tail Q(u) = P(u) exp(-u^2 / 2) for u >= 0, P a polynomial in 1 / (1 + 0.26 u) fitted to
+// erfc(u / sqrt 2) exp(u^2 / 2) / 2 (least squares, reweighted towards the smallest largest error): |error| < 2.2e-7 in
+// float32 arithmetic.  A third of the instructions of erff, whose two branches both run in most waves.
+// tail returns Q, e = exp(-u^2 / 2).
+__device__ __forceinline__ float normal_tail(float u, float& e) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.26f, u, 1.0f));
+  float p = fmaf(-0.07304021f, t, 0.22896615f);
+  p = fmaf(p, t, -0.10594359f);
+  p = fmaf(p, t, 0.16563688f);
+  p = fmaf(p, t, 0.07380697f);
+  p = fmaf(p, t, 0.10704367f);
+  p = fmaf(p, t, 0.10353009f);
+  e = __builtin_amdgcn_exp2f(u * u * -0.72134752f);
+  return p * t * e;
+}
+__device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
+
 __device__ __forceinline__ float activate(float z, int act) {
   switch (act) {
     case DISN_ACT_RELU: return z < 0.0f ? 0.0f : z;   // NaN stays
-    case DISN_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    case DISN_ACT_SILU: return z / (1.0f + expf(-z));
+    case DISN_ACT_GELU: {
+      float e;
+      const float q = normal_tail(fabsf(z), e);
+      return z * (z > 0.0f ? 1.0f - q : q);
+    }
+    case DISN_ACT_SILU: return z * logistic(z);
     default: return z;
   }
 }
@@ -55,11 +76,14 @@ __device__ __forceinline__ void activate_all(float (&z)[N], int act) {
 __device__ __forceinline__ float slope(float z, int act) {
   switch (act) {
     case DISN_ACT_RELU: return z > 0.0f ? 1.0f : z <= 0.0f ? 0.0f : z;
-    case DISN_ACT_GELU:
-      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * (0.39894228040143268f * expf(-0.5f * z * z));
+    case DISN_ACT_GELU: {
+      float e;
+      const float q = normal_tail(fabsf(z), e);
+      return fmaf(z * 0.39894228f, e, z > 0.0f ? 1.0f - q : q);
+    }
     case DISN_ACT_SILU: {
-      const float s = 1.0f / (1.0f + expf(-z));
-      return s * (1.0f + z * (1.0f - s));
+      const float s = logistic(z);
+      return s * fmaf(z, 1.0f - s, 1.0f);
     }
     default: return 1.0f;
   }
@@ -106,11 +130,11 @@ __device__ __forceinline__ void finish_vec(const Epilogue& e, int64_t row, int c
 }
 template <typename T>
 __device__ __forceinline__ Vec<T> bias_vec(const Epilogue& e, int col, int n) {
-  return e.bias && n > 0 ? load_vec((const T*)e.bias + col, n) : Vec<T>{};
+  return e.bias && n > 0 ? load_vec((const T*)e.bias + col, n, col) : Vec<T>{};
 }
 template <typename T>
 __device__ __forceinline__ Vec<T> residual_vec(const Epilogue& e, int64_t row, int col, int n) {
-  return e.residual && n > 0 ? load_vec((const T*)e.residual + row * e.ldr + col, n) : Vec<T>{};
+  return e.residual && n > 0 ? load_vec((const T*)e.residual + row * e.ldr + col, n, col) : Vec<T>{};
 }
 
 // Sums the partial products of a split r (0 of them: an empty sum) and finishes them.  A thread takes 16 bytes of the
@@ -194,40 +218,39 @@ __device__ __forceinline__ void tile_end(const TileArgs& a, int split, int iw, i
     return;
   }
   // Memory operations of a wave end in order, so a wait for a load is a wait for the stores before it: the bias is read
-  // once, the next rows' residual before the present rows are stored.
-  constexpr int W = NB * 32, V = Vec<T>::N, STRIDE = tile_stride(NB), Q = 32 * W / V / 64;
-  const int r0 = lane / (W / V), c = lane % (W / V) * V, j = jw + c, n_j = a.N - j;
+  // once, the residual two pieces ahead.  The loops stay loops: unrolled, they are 80 KB of code.
+  constexpr int W = NB * 32, V = Vec<T>::N, STRIDE = tile_stride(NB), Q = 32 * W / V / 64, STEP = 64 / (W / V);
+  const int c = lane % (W / V) * V, j = jw + c, n_j = a.N - j, r0 = lane / (W / V);
   const Vec<T> bias = bias_vec<T>(a.e, j, n_j);
-  Vec<T> res[2][Q];
-  auto read_residual = [&](int m) {
-#pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const int i = iw + m * 32 + r0 + q * (64 / (W / V));
-      res[m & 1][q] = residual_vec<T>(a.e, i, j, i < a.M ? n_j : 0);
-    }
-  };
-  read_residual(0);
+  const int i_end = min(a.M, iw + MB * 32);
+  Vec<T> res[2];   // this piece's and the next one's
+  res[0] = residual_vec<T>(a.e, iw + r0, j, iw + r0 < i_end ? n_j : 0);
+  res[1] = residual_vec<T>(a.e, iw + r0 + STEP, j, iw + r0 + STEP < i_end ? n_j : 0);
   __syncthreads();
   float* mine = lds + wave * (32 * STRIDE);
-#pragma unroll
-  for (int m = 0; m < MB; ++m) {
+#pragma unroll 1
+  for (int mm = 0; mm < MB; ++mm) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+    for (int m = 0; m < MB; ++m)
+      if (m == mm) {
 #pragma unroll
-      for (int g = 0; g < 16; ++g) mine[(ci + (g & 3) + 8 * (g >> 2)) * STRIDE + n * 32 + cj] = acc[m][n][g];
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int g = 0; g < 16; ++g) mine[(ci + (g & 3) + 8 * (g >> 2)) * STRIDE + n * 32 + cj] = acc[m][n][g];
+      }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    float z[Q][V];
-#pragma unroll
-    for (int q = 0; q < Q; ++q)
-      __builtin_memcpy(z[q], __builtin_assume_aligned(mine + (r0 + q * (64 / (W / V))) * STRIDE + c, 16), sizeof z[q]);
-    if (m + 1 < MB) read_residual(m + 1);
-#pragma unroll
+#pragma unroll 1
     for (int q = 0; q < Q; ++q) {
-      const int i = iw + m * 32 + r0 + q * (64 / (W / V));
-      if (i < a.M && n_j > 0) finish_vec<T>(a.e, i, j, z[q], n_j, bias, res[m & 1][q]);
+      const int r = r0 + q * STEP, i = iw + mm * 32 + r, ahead = i + 2 * STEP;
+      float z[V];
+      __builtin_memcpy(z, __builtin_assume_aligned(mine + r * STRIDE + c, 16), sizeof z);
+      const Vec<T> now = res[0];
+      res[0] = res[1];
+      res[1] = residual_vec<T>(a.e, ahead, j, ahead < i_end ? n_j : 0);
+      if (i < i_end && n_j > 0) finish_vec<T>(a.e, i, j, z, n_j, bias, now);
     }
   }
 }
@@ -292,11 +315,13 @@ struct Operand {
   const T* ptr[Q];
   int64_t ld;
   int left;          // i values in the tile
+  int first;         // the stage's first value in its row
   Vec<T> reg[Q];
 
   __device__ __forceinline__ void init(const T* p, int64_t ld_, int i0, int n_i, int64_t k0) {
     ld = ld_;
     left = n_i - i0;
+    first = ACROSS ? i0 : (int)k0;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int t = threadIdx.x + q * THREADS, line = t / PER_LINE, c = t % PER_LINE * V;
@@ -317,15 +342,15 @@ struct Operand {
       for (int q = 0; q < Q; ++q) {
         const int t = threadIdx.x + q * THREADS, line = t / PER_LINE, c = t % PER_LINE * V;
         if (ACROSS) {
-          const int n = c < left ? left - c : left;
-          reg[q] = load_vec(ptr[q] - (line < have ? 0 : line * ld), line < have ? n : 0);
+          reg[q] = load_vec(ptr[q] - (line < have ? 0 : line * ld), line < have ? (c < left ? left - c : left) : 0, first + (c < left ? c : 0));
         } else {
-          reg[q] = load_vec(ptr[q] - (c < have ? 0 : c), have - c);
+          reg[q] = load_vec(ptr[q] - (c < have ? 0 : c), have - c, first + c);
         }
       }
     }
 #pragma unroll
     for (int q = 0; q < Q; ++q) ptr[q] += ACROSS ? KT * ld : KT;
+    if (!ACROSS) first += KT;
   }
   __device__ __forceinline__ void store(char* lds) const {
 #pragma unroll
@@ -489,7 +514,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_tile(TileArgs a) {
 // bytes), and the four pieces of a row are exchanged by (i >> 2) & 3: sixteen lanes of a fragment, sixteen rows, touch
 // all 64 banks.  Across r it holds [r][i], pieces exchanged by (r & 3) << 2: the four rows that 32 lanes read through
 // ds_read_b64_tr_b16, 64 bytes of each, lie on different banks.  Needs operands on 16-byte boundaries; others are copied first
-// (k_pack).  The last stage, where r is not a multiple of 32, goes through registers, with zeros behind it.
+// (k_pack).  Where r is not a multiple of 32, the rest goes through registers into a fifth slot, with zeros behind it.
 constexpr int KT16 = 32, RING = 4;
 template <typename T, bool ACROSS, int ROWS, int WAVES, int BLOCKS>
 struct Operand16 {
@@ -498,7 +523,8 @@ struct Operand16 {
   const char* base;        // uniform: the stage to come
   int64_t step;            // bytes between stages
   unsigned off[PIECES];    // this lane's piece, relative to base
-  int left;
+  int left;                // i values in the tile
+  int first;               // the first stage's first value in its row
 
   __device__ __forceinline__ static int line_of(int p) { return ((threadIdx.x >> 6) * PIECES + p) * (64 / PER_LINE) + (threadIdx.x & 63) / PER_LINE; }
   __device__ __forceinline__ static int piece_of(int line) {
@@ -506,6 +532,7 @@ struct Operand16 {
   }
   __device__ __forceinline__ void init(const void* p, int64_t ld, int i0, int n_i, int64_t k0) {
     left = n_i - i0;
+    first = ACROSS ? i0 : (int)k0;
     base = (const char*)p + (ACROSS ? k0 * ld + i0 : (int64_t)i0 * ld + k0) * 2;
     step = (ACROSS ? KT16 * ld : KT16) * 2;
 #pragma unroll
@@ -515,28 +542,30 @@ struct Operand16 {
       off[p] = ACROSS ? (unsigned)(line * ld + (c < left ? c : 0)) * 2 : (unsigned)((line < left ? line : left - 1) * ld + c) * 2;
     }
   }
-  // the next stage into LDS at dst; have: how many r values exist from it on
-  __device__ __forceinline__ void fetch(char* dst, int have) {
-    dst += (threadIdx.x >> 6) * (PIECES * 1024);
-    if (have >= KT16) {
-      const unsigned m0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(lds_char*)dst);
+  // the next stage into LDS at dst
+  __device__ __forceinline__ void fetch(char* dst) {
+    const unsigned m0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(lds_char*)dst) + (threadIdx.x >> 6) * (PIECES * 1024);
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(m0 + p * 1024), "v"(off[p]), "s"(base) : "memory");
-    } else {
-#pragma unroll
-      for (int p = 0; p < PIECES; ++p) {
-        const int line = line_of(p), c = piece_of(line) * 8;
-        const T* src = (const T*)(base + off[p]);
-        Vec<T> v;
-        if (ACROSS)
-          v = load_vec(line < have ? src : (const T*)base, line < have ? (c < left ? left - c : left) : 0);
-        else
-          v = load_vec(c < have ? src : (const T*)base, have - c);
-        __builtin_memcpy(__builtin_assume_aligned(dst + p * 1024 + (threadIdx.x & 63) * 16, 16), &v, 16);
-      }
-    }
+    for (int p = 0; p < PIECES; ++p)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(m0 + p * 1024)),
+                   "v"(off[p]), "s"(base)
+                   : "memory");
     base += step;
+  }
+  // stage t, of which only the first `have` r values exist, through registers: zeros behind them
+  __device__ __forceinline__ void fetch_part(char* dst, const char* first_stage, int t, int have) const {
+    const char* from = first_stage + t * step;
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+      const int line = line_of(p), c = piece_of(line) * 8;
+      const T* src = (const T*)(from + off[p]);
+      Vec<T> v;
+      if (ACROSS)
+        v = load_vec(line < have ? src : (const T*)from, line < have ? (c < left ? left - c : left) : 0, first + (c < left ? c : 0));
+      else
+        v = load_vec(c < have ? src : (const T*)from, have - c, first + t * KT16 + c);
+      __builtin_memcpy(__builtin_assume_aligned(dst + ((threadIdx.x >> 6) * PIECES + p) * 1024 + (threadIdx.x & 63) * 16, 16), &v, 16);
+    }
   }
   // byte offsets of this lane's part of a wave's fragments, whose i values start at iw (a multiple of 32): along r one for
   // each step of 16 r, across r one for each block of 32 i
@@ -579,7 +608,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_tile16(TileArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const TilePlace at = tile_place(a, BM, BN);
   const int64_t k0 = at.split * a.per;
-  const int have = (int)(a.K - k0 < a.per ? a.K - k0 : a.per), stages = (have + KT16 - 1) / KT16, whole = have / KT16;
+  const int have = (int)(a.K - k0 < a.per ? a.K - k0 : a.per), stages = have / KT16, rest = have % KT16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WN * (MB * 32), wj = wave % WN * (NB * 32);
 
   floatx16 acc[MB][NB];
@@ -596,20 +625,21 @@ __global__ __launch_bounds__(WM * WN * 64) void k_tile16(TileArgs a) {
   unsigned oa[OpA::OFFSETS], ob[OpB::OFFSETS];
   OpA::lane_offsets(wi, oa);
   OpB::lane_offsets(wj, ob);
+  const char *a0 = A.base, *b0 = B.base;
   auto fetch = [&](int t) {
     if (t >= stages) return;
     char* dst = lds + (t & (RING - 1)) * BUF;
-    A.fetch(dst, have - t * KT16);
-    B.fetch(dst + OpA::BYTES, have - t * KT16);
+    A.fetch(dst);
+    B.fetch(dst + OpA::BYTES);
   };
   shortx8 fa[2][MB], fb[2][NB];
-  auto read = [&](int t, int s) {
-    const char* p = lds + (t & (RING - 1)) * BUF;
+  auto read_at = [&](const char* p, int s) {
 #pragma unroll
     for (int n = 0; n < NB; ++n) fb[s][n] = OpB::fragment(p + OpA::BYTES, ob, n, s);
 #pragma unroll
     for (int m = 0; m < MB; ++m) fa[s][m] = OpA::fragment(p, oa, m, s);
   };
+  auto read = [&](int t, int s) { read_at(lds + (t & (RING - 1)) * BUF, s); };
   auto multiply = [&](int s) {
 #pragma unroll
     for (int m = 0; m < MB; ++m)
@@ -617,27 +647,38 @@ __global__ __launch_bounds__(WM * WN * 64) void k_tile16(TileArgs a) {
       for (int n = 0; n < NB; ++n) acc[m][n] = mfma<T>(fa[s][m], fb[s][n], acc[m][n]);
   };
   // stage t has landed for everyone, and everyone has read what it wants of the stage before.  Stages up to t + 2 are
-  // under way, four loads of this wave each (the last, partial one has none).
+  // under way, four loads of this wave each.
   auto meet = [&](int t) {
-    const int behind = min(t + 3, whole) - (t + 1);
+    const int behind = min(t + 3, stages) - (t + 1);
     if (behind >= 2) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     else if (behind == 1) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
-  fetch(0);
-  fetch(1);
-  fetch(2);
+#pragma unroll 1
+  for (int t = 0; t < 3; ++t) fetch(t);
+  if (rest) {   // the last, partial stage waits in a slot of its own
+    A.fetch_part(lds + RING * BUF, a0, stages, rest);
+    B.fetch_part(lds + RING * BUF + OpA::BYTES, b0, stages, rest);
+  }
   meet(0);
-  fetch(3);
-  read(0, 0);
-  for (int t = 0; t < stages; ++t) {
-    read(t, 1);
-    multiply(0);
-    if (t + 1 < stages) {
-      meet(t + 1);
-      fetch(t + 4);
-      read(t + 1, 0);
+  if (stages) {
+    fetch(3);
+    read(0, 0);
+    for (int t = 0; t < stages; ++t) {
+      read(t, 1);
+      multiply(0);
+      if (t + 1 < stages) {
+        meet(t + 1);
+        fetch(t + 4);
+        read(t + 1, 0);
+      }
+      multiply(1);
     }
+  }
+  if (rest) {
+    read_at(lds + RING * BUF, 0);
+    multiply(0);
+    read_at(lds + RING * BUF, 1);
     multiply(1);
   }
   tile_end<T, MB, NB, WAVES>(a, at.split, at.i0 + wi, at.j0 + wj, acc, (float*)lds);
@@ -650,7 +691,7 @@ __global__ __launch_bounds__(256) void k_pack(const T* __restrict__ src, int64_t
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
     const int64_t r = t / per;
     const int c = (int)(t - r * per) * 8;
-    const Vec<T> v = load_vec(src + r * lds_ + c, cols - c);
+    const Vec<T> v = load_vec(src + r * lds_ + c, cols - c, c);
     store_vec(dst + r * ldd + c, v, 8);
   }
 }
@@ -850,9 +891,9 @@ __global__ __launch_bounds__(256) void k_rows_across(RowsArgs a) {
 #pragma unroll
       for (int u = 0; u < 8; ++u) add(k + 4 * u, v[u]);
     }
-    for (; k < have; k += 4) add(k, load_vec(w + (int64_t)k * a.ldw, wide ? V : a.N));
+    for (; k < have; k += 4) add(k, load_vec(w + (int64_t)k * a.ldw, wide ? V : a.N, 0));
   } else {
-    for (int k = wave; k < have; k += 4) add(k, load_vec(w + (int64_t)k * a.ldw, n));
+    for (int k = wave; k < have; k += 4) add(k, load_vec(w + (int64_t)k * a.ldw, n, col));
   }
 #pragma unroll
   for (int m = 0; m < MR; ++m) {
@@ -885,10 +926,10 @@ __global__ __launch_bounds__(256) void k_rows_along(RowsArgs a) {
     const int n = a.K - k;
     Vec<T> wv[NR];
 #pragma unroll
-    for (int j = 0; j < NR; ++j) wv[j] = load_vec(w[j] + k, n);
+    for (int j = 0; j < NR; ++j) wv[j] = load_vec(w[j] + k, n, k);
 #pragma unroll
     for (int m = 0; m < MR; ++m) {
-      const Vec<T> xv = load_vec((const T*)a.x + min(m, a.M - 1) * a.ldx + k, n);
+      const Vec<T> xv = load_vec((const T*)a.x + min(m, a.M - 1) * a.ldx + k, n, k);
 #pragma unroll
       for (int j = 0; j < NR; ++j)
 #pragma unroll
@@ -936,12 +977,12 @@ __global__ __launch_bounds__(256) void k_gate(GateArgs a) {
   if (n > 0) {
 #pragma unroll 4
     for (int64_t r = rb * a.rows_per + line; r < r1; r += lines) {
-      const Vec<T> g = load_vec((const T*)a.dy + r * a.lddy + col, n);
+      const Vec<T> g = load_vec((const T*)a.dy + r * a.lddy + col, n, col);
       float v[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] = (float)g.v[i];
       if (a.act != DISN_ACT_NONE) {
-        const Vec<T> z = load_vec((const T*)a.pre + r * a.ldp + col, n);
+        const Vec<T> z = load_vec((const T*)a.pre + r * a.ldp + col, n, col);
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] *= slope((float)z.v[i], a.act);
       }
@@ -1042,13 +1083,15 @@ template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int 
 int launch_tile(DisnCtx* ctx, const TileArgs& a, hipStream_t stream) {
   constexpr int THREADS = WM * WN * 64;
   const void* kernel;
-  int bytes;
+  int bytes, used;
   if constexpr (sizeof(T) == 4) {
     kernel = (const void*)k_tile<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN>;
     bytes = 2 * (Operand<T, A_ACROSS, BM, THREADS>::BYTES + Operand<T, B_ACROSS, BN, THREADS>::BYTES);
+    used = bytes;
   } else {
     kernel = (const void*)k_tile16<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN>;
-    bytes = RING * (BM + BN) * KT16 * 2;
+    bytes = (RING + 1) * (BM + BN) * KT16 * 2;   // the fifth slot is allocated only where r leaves a rest
+    used = (RING + (a.K % KT16 ? 1 : 0)) * (BM + BN) * KT16 * 2;
   }
   static std::atomic<uint64_t> ready{0};   // devices that allow this kernel its LDS
   const uint64_t bit = 1ull << (ctx->device & 63);
@@ -1058,7 +1101,7 @@ int launch_tile(DisnCtx* ctx, const TileArgs& a, hipStream_t stream) {
   }
   TileArgs copy = a;
   void* args[] = {&copy};
-  DISN_HIP(ctx, hipLaunchKernel(kernel, dim3((unsigned)((int64_t)a.mt * a.nt * a.splits)), dim3(THREADS), args, bytes, stream));
+  DISN_HIP(ctx, hipLaunchKernel(kernel, dim3((unsigned)((int64_t)a.mt * a.nt * a.splits)), dim3(THREADS), args, used, stream));
   return DISN_OK;
 }
 template <typename T, bool A_ACROSS, bool B_ACROSS>

@@ -57,7 +57,7 @@ __device__ __forceinline__ void load_row(const T* row, int t, int d, Vec<T> (&ou
 #pragma unroll
   for (int p = 0; p < E / Vec<T>::N; ++p) {
     const int c = piece_col<T, G>(t, p);
-    out[p] = load_vec(row + (c < d ? c : 0), c < d ? d - c : 0);
+    out[p] = load_vec(row + (c < d ? c : 0), c < d ? d - c : 0, c);
   }
 }
 
@@ -70,8 +70,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm(NormArgs a) {
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     const int c = piece_col<T, G>(t, p), n = c < d ? d - c : 0;
-    const Vec<T> wv = a.weight ? load_vec((const T*)a.weight + (n ? c : 0), n) : Vec<T>{};
-    const Vec<T> bv = a.bias ? load_vec((const T*)a.bias + (n ? c : 0), n) : Vec<T>{};
+    const Vec<T> wv = a.weight ? load_vec((const T*)a.weight + (n ? c : 0), n, c) : Vec<T>{};
+    const Vec<T> bv = a.bias ? load_vec((const T*)a.bias + (n ? c : 0), n, c) : Vec<T>{};
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       w[p * N + i] = a.weight ? (float)wv.v[i] : 1.0f;
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm_backward(NormA
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     const int c = piece_col<T, G>(t, p), n = c < d ? d - c : 0;
-    const Vec<T> wv = a.weight ? load_vec((const T*)a.weight + (n ? c : 0), n) : Vec<T>{};
+    const Vec<T> wv = a.weight ? load_vec((const T*)a.weight + (n ? c : 0), n, c) : Vec<T>{};
 #pragma unroll
     for (int i = 0; i < N; ++i) w[p * N + i] = a.weight ? (float)wv.v[i] : 1.0f;
   }
