@@ -505,17 +505,17 @@ __global__ __launch_bounds__(WM * WN * 64) void k_tile(TileArgs a) {
 }
 
 // ---- k_tile16 ------------------------------------------------------------------------------------------------------
-// bf16 and fp16.  A ring of four LDS stages of 32 r is filled by DMA (global_load_lds_dwordx4: no registers, no LDS
-// store instructions), so three stages, 96 KB a CU with 256-wide tiles, are on their way while one is multiplied.  Two
-// steps of 16 r a stage, and the fragments of a step are read while the step before is multiplied; the one barrier of a
-// stage lies between its two steps, when the second step's fragments are in registers: no wave waits for LDS behind it.
+// bf16 and fp16.  A ring of LDS stages of 32 r is filled by DMA (global_load_lds_dwordx4: no registers, no LDS store
+// instructions), so all but one of its stages are on their way while one is multiplied.  Two steps of 16 r a stage, and
+// the fragments of a step are read while the step before is multiplied; the one barrier of a stage lies between its two
+// steps, when the second step's fragments are in registers: no wave waits for LDS behind it.
 //
 // A wave's DMA writes 1 KB of LDS in lane order, from any 16-byte pieces of memory.  Along r, LDS holds [i][32 r] (64
 // bytes), and the four pieces of a row are exchanged by (i >> 2) & 3: sixteen lanes of a fragment, sixteen rows, touch
 // all 64 banks.  Across r it holds [r][i], pieces exchanged by (r & 3) << 2: the four rows that 32 lanes read through
-// ds_read_b64_tr_b16, 64 bytes of each, lie on different banks.  Needs operands on 16-byte boundaries; others are copied first
-// (k_pack).  Where r is not a multiple of 32, the rest goes through registers into a fifth slot, with zeros behind it.
-constexpr int KT16 = 32, RING = 4;
+// ds_read_b64_tr_b16, 64 bytes of each, lie on different banks.  Needs operands on 16-byte boundaries; others are copied
+// first (k_pack).  In the last stage, where r is not a multiple of 32, every lane clears what it has fetched behind the end.
+constexpr int KT16 = 32;
 template <typename T, bool ACROSS, int ROWS, int WAVES, int BLOCKS>
 struct Operand16 {
   static constexpr int BYTES = ROWS * KT16 * 2, PIECES = BYTES / 1024 / WAVES, PER_LINE = (ACROSS ? ROWS : KT16) / 8;
@@ -523,16 +523,15 @@ struct Operand16 {
   const char* base;        // uniform: the stage to come
   int64_t step;            // bytes between stages
   unsigned off[PIECES];    // this lane's piece, relative to base
-  int left;                // i values in the tile
-  int first;               // the first stage's first value in its row
+  unsigned line_bytes;
 
   __device__ __forceinline__ static int line_of(int p) { return ((threadIdx.x >> 6) * PIECES + p) * (64 / PER_LINE) + (threadIdx.x & 63) / PER_LINE; }
   __device__ __forceinline__ static int piece_of(int line) {
     return ((threadIdx.x & 63) % PER_LINE) ^ (ACROSS ? (line & 3) << 2 : (line >> 2) & 3);
   }
   __device__ __forceinline__ void init(const void* p, int64_t ld, int i0, int n_i, int64_t k0) {
-    left = n_i - i0;
-    first = ACROSS ? i0 : (int)k0;
+    const int left = n_i - i0;
+    line_bytes = (unsigned)ld * 2;
     base = (const char*)p + (ACROSS ? k0 * ld + i0 : (int64_t)i0 * ld + k0) * 2;
     step = (ACROSS ? KT16 * ld : KT16) * 2;
 #pragma unroll
@@ -542,29 +541,31 @@ struct Operand16 {
       off[p] = ACROSS ? (unsigned)(line * ld + (c < left ? c : 0)) * 2 : (unsigned)((line < left ? line : left - 1) * ld + c) * 2;
     }
   }
-  // the next stage into LDS at dst
-  __device__ __forceinline__ void fetch(char* dst) {
-    const unsigned m0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(lds_char*)dst) + (threadIdx.x >> 6) * (PIECES * 1024);
-#pragma unroll
-    for (int p = 0; p < PIECES; ++p)
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(m0 + p * 1024)),
-                   "v"(off[p]), "s"(base)
-                   : "memory");
-    base += step;
-  }
-  // stage t, of which only the first `have` r values exist, through registers: zeros behind them
-  __device__ __forceinline__ void fetch_part(char* dst, const char* first_stage, int t, int have) const {
-    const char* from = first_stage + t * step;
+  // the next stage into LDS at dst; have: r values that exist from it on.  Pieces wholly behind the end come from the
+  // stage's first one; a piece that holds the end is read whole (16 aligned bytes never leave the memory of their first)
+  __device__ __forceinline__ void fetch(char* dst, int have) {
+    const unsigned m0 = (unsigned)(size_t)(lds_char*)dst + (threadIdx.x >> 6) * (PIECES * 1024);
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-      const int line = line_of(p), c = piece_of(line) * 8;
-      const T* src = (const T*)(from + off[p]);
-      Vec<T> v;
-      if (ACROSS)
-        v = load_vec(line < have ? src : (const T*)from, line < have ? (c < left ? left - c : left) : 0, first + (c < left ? c : 0));
-      else
-        v = load_vec(c < have ? src : (const T*)from, have - c, first + t * KT16 + c);
-      __builtin_memcpy(__builtin_assume_aligned(dst + ((threadIdx.x >> 6) * PIECES + p) * 1024 + (threadIdx.x & 63) * 16, 16), &v, 16);
+      const int line = line_of(p);
+      const bool in = have >= KT16 || (ACROSS ? line : piece_of(line) * 8) < have;
+      const unsigned o = in ? off[p] : off[p] - (ACROSS ? line * line_bytes : (unsigned)piece_of(line) * 16);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(m0 + p * 1024)),
+                   "v"(o), "s"(base)
+                   : "memory");
+    }
+    base += step;
+  }
+  // clears this lane's values behind the end of a landed stage
+  __device__ __forceinline__ static void clear(char* dst, int have) {
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+      const int line = line_of(p), n = ACROSS ? (line < have ? 8 : 0) : have - piece_of(line) * 8;
+      if (n >= 8) continue;
+      T* at = (T*)(dst + ((threadIdx.x >> 6) * PIECES + p) * 1024 + (threadIdx.x & 63) * 16);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i >= n) at[i] = (T)0.0f;
     }
   }
   // byte offsets of this lane's part of a wave's fragments, whose i values start at iw (a multiple of 32): along r one for
@@ -597,18 +598,18 @@ struct Operand16 {
   }
 };
 
-template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN>
+template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int RING>
 __global__ __launch_bounds__(WM * WN * 64) void k_tile16(TileArgs a) {
   constexpr int WAVES = WM * WN, MB = BM / WM / 32, NB = BN / WN / 32;
   typedef Operand16<T, A_ACROSS, BM, WAVES, MB> OpA;
   typedef Operand16<T, B_ACROSS, BN, WAVES, NB> OpB;
   constexpr int BUF = OpA::BYTES + OpB::BYTES, LOADS = OpA::PIECES + OpB::PIECES;
   static_assert(32 * tile_stride(NB) * 4 * WAVES <= RING * BUF, "the turned tiles fit into the ring");
-  static_assert(LOADS == 4, "waits count four loads a stage");
+  static_assert(RING == 3 || RING == 4, "waits");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const TilePlace at = tile_place(a, BM, BN);
   const int64_t k0 = at.split * a.per;
-  const int have = (int)(a.K - k0 < a.per ? a.K - k0 : a.per), stages = have / KT16, rest = have % KT16;
+  const int have = (int)(a.K - k0 < a.per ? a.K - k0 : a.per), whole = have / KT16, rest = have % KT16, stages = whole + (rest ? 1 : 0);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WN * (MB * 32), wj = wave % WN * (NB * 32);
 
   floatx16 acc[MB][NB];
@@ -625,60 +626,59 @@ __global__ __launch_bounds__(WM * WN * 64) void k_tile16(TileArgs a) {
   unsigned oa[OpA::OFFSETS], ob[OpB::OFFSETS];
   OpA::lane_offsets(wi, oa);
   OpB::lane_offsets(wj, ob);
-  const char *a0 = A.base, *b0 = B.base;
+  auto slot = [&](int t) { return lds + (RING == 4 ? t & 3 : t % 3) * BUF; };
   auto fetch = [&](int t) {
     if (t >= stages) return;
-    char* dst = lds + (t & (RING - 1)) * BUF;
-    A.fetch(dst);
-    B.fetch(dst + OpA::BYTES);
+    A.fetch(slot(t), have - t * KT16);
+    B.fetch(slot(t) + OpA::BYTES, have - t * KT16);
   };
   shortx8 fa[2][MB], fb[2][NB];
-  auto read_at = [&](const char* p, int s) {
+  auto read = [&](int t, int s) {
+    const char* p = slot(t);
 #pragma unroll
     for (int n = 0; n < NB; ++n) fb[s][n] = OpB::fragment(p + OpA::BYTES, ob, n, s);
 #pragma unroll
     for (int m = 0; m < MB; ++m) fa[s][m] = OpA::fragment(p, oa, m, s);
   };
-  auto read = [&](int t, int s) { read_at(lds + (t & (RING - 1)) * BUF, s); };
   auto multiply = [&](int s) {
 #pragma unroll
     for (int m = 0; m < MB; ++m)
 #pragma unroll
       for (int n = 0; n < NB; ++n) acc[m][n] = mfma<T>(fa[s][m], fb[s][n], acc[m][n]);
   };
-  // stage t has landed for everyone, and everyone has read what it wants of the stage before.  Stages up to t + 2 are
-  // under way, four loads of this wave each.
+  // stage t has landed for everyone, and everyone has read what it wants of the stage before.  Stages up to
+  // t + RING - 2 are under way, LOADS loads of this wave each.
   auto meet = [&](int t) {
-    const int behind = min(t + 3, stages) - (t + 1);
-    if (behind >= 2) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    else if (behind == 1) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const int behind = min(t + RING - 1, stages) - (t + 1);
+    if (RING == 4 && behind >= 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
+    else if (behind >= 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
 #pragma unroll 1
-  for (int t = 0; t < 3; ++t) fetch(t);
-  if (rest) {   // the last, partial stage waits in a slot of its own
-    A.fetch_part(lds + RING * BUF, a0, stages, rest);
-    B.fetch_part(lds + RING * BUF + OpA::BYTES, b0, stages, rest);
-  }
-  meet(0);
-  if (stages) {
-    fetch(3);
+  for (int t = 0; t < RING - 1; ++t) fetch(t);
+  if (whole) {
+    meet(0);
+    fetch(RING - 1);
     read(0, 0);
-    for (int t = 0; t < stages; ++t) {
+    for (int t = 0; t < whole; ++t) {
       read(t, 1);
       multiply(0);
-      if (t + 1 < stages) {
+      if (t + 1 < whole) {
         meet(t + 1);
-        fetch(t + 4);
+        fetch(t + RING);
         read(t + 1, 0);
       }
       multiply(1);
     }
   }
   if (rest) {
-    read_at(lds + RING * BUF, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    OpA::clear(slot(whole), rest);
+    OpB::clear(slot(whole) + OpA::BYTES, rest);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    read(whole, 0);
     multiply(0);
-    read_at(lds + RING * BUF, 1);
+    read(whole, 1);
     multiply(1);
   }
   tile_end<T, MB, NB, WAVES>(a, at.split, at.i0 + wi, at.j0 + wj, acc, (float*)lds);
@@ -1079,19 +1079,17 @@ int launch_finish(DisnCtx* ctx, const float* part, int nparts, int64_t M, int64_
   return DISN_OK;
 }
 
-template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN>
+template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int RING>
 int launch_tile(DisnCtx* ctx, const TileArgs& a, hipStream_t stream) {
   constexpr int THREADS = WM * WN * 64;
   const void* kernel;
-  int bytes, used;
+  int bytes;
   if constexpr (sizeof(T) == 4) {
     kernel = (const void*)k_tile<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN>;
     bytes = 2 * (Operand<T, A_ACROSS, BM, THREADS>::BYTES + Operand<T, B_ACROSS, BN, THREADS>::BYTES);
-    used = bytes;
   } else {
-    kernel = (const void*)k_tile16<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN>;
-    bytes = (RING + 1) * (BM + BN) * KT16 * 2;   // the fifth slot is allocated only where r leaves a rest
-    used = (RING + (a.K % KT16 ? 1 : 0)) * (BM + BN) * KT16 * 2;
+    kernel = (const void*)k_tile16<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN, RING>;
+    bytes = RING * (BM + BN) * KT16 * 2;
   }
   static std::atomic<uint64_t> ready{0};   // devices that allow this kernel its LDS
   const uint64_t bit = 1ull << (ctx->device & 63);
@@ -1101,13 +1099,13 @@ int launch_tile(DisnCtx* ctx, const TileArgs& a, hipStream_t stream) {
   }
   TileArgs copy = a;
   void* args[] = {&copy};
-  DISN_HIP(ctx, hipLaunchKernel(kernel, dim3((unsigned)((int64_t)a.mt * a.nt * a.splits)), dim3(THREADS), args, used, stream));
+  DISN_HIP(ctx, hipLaunchKernel(kernel, dim3((unsigned)((int64_t)a.mt * a.nt * a.splits)), dim3(THREADS), args, bytes, stream));
   return DISN_OK;
 }
 template <typename T, bool A_ACROSS, bool B_ACROSS>
 int launch_tile(DisnCtx* ctx, int tile, const TileArgs& a, hipStream_t stream) {
-  return tile == 256 ? launch_tile<T, A_ACROSS, B_ACROSS, 256, 256, 2, 4>(ctx, a, stream)
-                     : launch_tile<T, A_ACROSS, B_ACROSS, 128, 128, 2, 2>(ctx, a, stream);
+  return tile == 256 ? launch_tile<T, A_ACROSS, B_ACROSS, 256, 256, 2, 4, 4>(ctx, a, stream)
+                     : launch_tile<T, A_ACROSS, B_ACROSS, 128, 128, 2, 2, 4>(ctx, a, stream);
 }
 // a copy of rows x cols values at dst, 16-byte boundaries; *p, *ld become it
 template <typename T>
