@@ -7,7 +7,7 @@
 // An operand lies "along" r (its r values are contiguous) or "across" (its i values are, rows of r).
 //
 // Three kernels compute it, chosen by size (plan() below):
-//   k_tile   large products: 128- or 256-wide tiles through LDS on the matrix cores
+//   k_tile16, k_tile32  large products: 128- or 256-wide tiles through LDS on the matrix cores
 //   k_small  products of a few tens of microseconds and less: no LDS tiles, the waves of a workgroup share the sum
 //   k_rows_* at most 16 rows times a large matrix: W streams past at memory speed
 #include "dense.h"
@@ -268,30 +268,21 @@ __device__ __forceinline__ TilePlace tile_place(const TileArgs& a, int BM, int B
   return {id % a.mt * BM, tn * BN, id / a.mt};
 }
 
-// ---- k_tile --------------------------------------------------------------------------------------------------------
+// ---- k_tile32 --------------------------------------------------------------------------------------------------------
 // A workgroup computes a BM x BN tile of C, r in stages of KT.  The stage after the next is on its way from memory to
 // registers while the next lies in one LDS buffer and the waves multiply the present one from the other: one barrier a
 // stage.  Waves are WM x WN; each has MB x NB tiles of v_mfma_f32_32x32x16.
 //
-// 16-bit types go to the matrix cores as they are.  fp32 is cut into three bf16 terms x = h + m + l (each the rounded
+// For fp32, which is cut into three bf16 terms x = h + m + l (each the rounded
 // rest of the one before; 8 + 8 + 8 bits hold fp32's 24, so the sum is exact) and the six products
 // hh, hm, mh, mm, hl, lh are accumulated in fp32; what is left out (ml, lm, ll) is below 2^-24 of a product, as an
 // FMA's rounding is.  Six bf16 MFMAs take 6/16 of the time of one fp32 MFMA of the same size.  Infinities,
 // NaN and intermediate overflow cannot be cut; a tile whose sums are not all finite is computed again by plain FMAs.
 //
-// LDS: an operand along r as [16 r][i][32 bytes] (a wave's fragment is 1 KB in one piece; 32 bytes between the 16-r
-// blocks put the eight lanes that store one row on different banks); an operand across r as [r][i] with 64 bytes
-// between rows, read through ds_read_b64_tr_b16, which hands each lane 4 r values of its i.
-template <typename T>
-struct Mma {
-  static constexpr int planes = 1;
-  static constexpr int KT = 64;
-};
-template <>
-struct Mma<float> {
-  static constexpr int planes = 3;
-  static constexpr int KT = 16;
-};
+// LDS: an operand along r as [8 r][i][16 bytes] (half a fragment is 512 bytes in one piece; 128 bytes between the 8-r
+// blocks put the lanes that store a row on different banks); an operand across r as [r][i] with 64 bytes between rows,
+// read through ds_read_b64_tr_b16, which hands each lane 4 r values of its i.
+constexpr int KT32 = 16, PLANES = 3;
 
 template <typename T>
 __device__ __forceinline__ floatx16 mfma(shortx8 a, shortx8 b, floatx16 c) {
@@ -303,12 +294,12 @@ __device__ __forceinline__ floatx16 mfma(shortx8 a, shortx8 b, floatx16 c) {
 
 template <typename T, bool ACROSS, int ROWS, int THREADS>
 struct Operand {
-  static constexpr int KT = Mma<T>::KT, P = Mma<T>::planes, V = Vec<T>::N;
+  static constexpr int KT = KT32, P = PLANES, V = Vec<T>::N;
   static constexpr int PER_LINE = (ACROSS ? ROWS : KT) / V;    // 16-byte pieces in a contiguous run
   static constexpr int Q = ROWS * KT / V / THREADS;            // pieces a thread moves per stage
   static constexpr int LINE = ROWS * 2 + 64;                   // bytes of one r (across)
-  static constexpr int BLOCK = ROWS * 32 + 32;                 // bytes of 16 r (along)
-  static constexpr int PLANE = ACROSS ? KT * LINE : KT / 16 * BLOCK;
+  static constexpr int BLOCK = ROWS * 16 + 128;                // bytes of 8 r (along)
+  static constexpr int PLANE = ACROSS ? KT * LINE : KT / 8 * BLOCK;
   static constexpr int BYTES = PLANE * P;
   static_assert(Q * THREADS * V == ROWS * KT, "pieces");
 
@@ -356,23 +347,19 @@ struct Operand {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int t = threadIdx.x + q * THREADS, line = t / PER_LINE, c = t % PER_LINE * V;
-      char* dst = lds + (ACROSS ? line * LINE + c * 2 : (c >> 4) * BLOCK + line * 32 + (c & 15) * 2);
-      if constexpr (P == 1) {
-        __builtin_memcpy(__builtin_assume_aligned(dst, 16), &reg[q], 16);
-      } else {
-        float rest[4];
+      char* dst = lds + (ACROSS ? line * LINE + c * 2 : (c >> 3) * BLOCK + line * 16 + (c & 7) * 2);
+      float rest[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) rest[i] = reg[q].v[i];
+      for (int i = 0; i < 4; ++i) rest[i] = reg[q].v[i];
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-          bf16_t term[4];
+      for (int p = 0; p < P; ++p) {
+        bf16_t term[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            term[i] = (bf16_t)rest[i];
-            rest[i] -= (float)term[i];
-          }
-          __builtin_memcpy(__builtin_assume_aligned(dst + p * PLANE, 8), term, 8);
+        for (int i = 0; i < 4; ++i) {
+          term[i] = (bf16_t)rest[i];
+          rest[i] -= (float)term[i];
         }
+        __builtin_memcpy(__builtin_assume_aligned(dst + p * PLANE, 8), term, 8);
       }
     }
   }
@@ -387,15 +374,45 @@ struct Operand {
       const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_shortx4*)(p + 4 * LINE));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-      const char* p = lds + plane * PLANE + s * BLOCK + (i + (lane & 31)) * 32 + (lane >> 5) * 16;
+      const char* p = lds + plane * PLANE + (2 * s + (lane >> 5)) * BLOCK + (i + (lane & 31)) * 16;
       return *(const shortx8*)p;
     }
   }
 };
 
+// a tile of fp32 by plain multiply-adds, eight rows of a column at a time
+__device__ __forceinline__ void fma_tile(const TileArgs& a, bool a_across, bool b_across, int bm, int bn, int threads, int i0, int j0, int split,
+                                      int64_t k0, int have) {
+  const int64_t ai = a_across ? 1 : a.lda, ar = a_across ? a.lda : 1, bj = b_across ? 1 : a.ldb, br = b_across ? a.ldb : 1;
+  for (int t = threadIdx.x; t < bm / 8 * bn; t += threads) {
+    const int i = i0 + t / bn * 8, j = j0 + t % bn;
+    if (i >= a.M || j >= a.N) continue;
+    const float* pa = (const float*)a.A + k0 * ar;
+    const float* pb = (const float*)a.B + j * bj + k0 * br;
+    float s[8];
+    int64_t row[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      s[q] = 0.0f;
+      row[q] = min(i + q, a.M - 1) * ai;
+    }
+    for (int k = 0; k < have; ++k) {
+      const float b = pb[k * br];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) s[q] = fmaf(pa[row[q] + k * ar], b, s[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      if (i + q >= a.M) break;
+      if (a.splits > 1) a.part[((size_t)split * a.M + i + q) * a.N + j] = s[q];
+      else finish_one<float>(a.e, i + q, j, s[q]);
+    }
+  }
+}
+
 template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void k_tile(TileArgs a) {
-  constexpr int THREADS = WM * WN * 64, MB = BM / WM / 32, NB = BN / WN / 32, KT = Mma<T>::KT, P = Mma<T>::planes;
+__global__ __launch_bounds__(WM * WN * 64, 2) void k_tile32(TileArgs a) {
+  constexpr int THREADS = WM * WN * 64, MB = BM / WM / 32, NB = BN / WN / 32, KT = KT32, P = PLANES;
   typedef Operand<T, A_ACROSS, BM, THREADS> OpA;
   typedef Operand<T, B_ACROSS, BN, THREADS> OpB;
   constexpr int BUF = OpA::BYTES + OpB::BYTES;
@@ -404,7 +421,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_tile(TileArgs a) {
   const int i0 = at.i0, j0 = at.j0, split = at.split;
   const int64_t k0 = split * a.per;
   const int have = (int)(a.K - k0 < a.per ? a.K - k0 : a.per), stages = (have + KT - 1) / KT;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
   const int wi = wave / WN * (MB * 32), wj = wave % WN * (NB * 32);
 
   floatx16 acc[MB][NB];
@@ -453,13 +470,11 @@ __global__ __launch_bounds__(WM * WN * 64) void k_tile(TileArgs a) {
         for (int p = 0; p < P; ++p) f[p] = OpA::fragment(cur, p, wi + m * 32, q);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          if constexpr (P == 3) {
-            acc[m][n] = mfma<T>(f[2], b[n][0], acc[m][n]);
-            acc[m][n] = mfma<T>(f[0], b[n][2], acc[m][n]);
-            acc[m][n] = mfma<T>(f[1], b[n][1], acc[m][n]);
-            acc[m][n] = mfma<T>(f[1], b[n][0], acc[m][n]);
-            acc[m][n] = mfma<T>(f[0], b[n][1], acc[m][n]);
-          }
+          acc[m][n] = mfma<T>(f[2], b[n][0], acc[m][n]);
+          acc[m][n] = mfma<T>(f[0], b[n][2], acc[m][n]);
+          acc[m][n] = mfma<T>(f[1], b[n][1], acc[m][n]);
+          acc[m][n] = mfma<T>(f[1], b[n][0], acc[m][n]);
+          acc[m][n] = mfma<T>(f[0], b[n][1], acc[m][n]);
           acc[m][n] = mfma<T>(f[0], b[n][0], acc[m][n]);
         }
       }
@@ -467,8 +482,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_tile(TileArgs a) {
   }
 
   static_assert(32 * tile_stride(NB) * 4 * WM * WN <= 2 * BUF, "the turned tiles fit into the stage buffers");
-  const int cj = lane & 31, ci = 4 * (lane >> 5);
-  if constexpr (P == 3) {
+  {
     bool bad = false;
 #pragma unroll
     for (int m = 0; m < MB; ++m)
@@ -477,30 +491,10 @@ __global__ __launch_bounds__(WM * WN * 64) void k_tile(TileArgs a) {
 #pragma unroll
         for (int g = 0; g < 16; ++g) bad |= !(fabsf(acc[m][n][g]) <= 3.4028235e38f);
     if (__syncthreads_or(bad)) {
-      const int64_t ai = A_ACROSS ? 1 : a.lda, ar = A_ACROSS ? a.lda : 1, bj = B_ACROSS ? 1 : a.ldb, br = B_ACROSS ? a.ldb : 1;
-#pragma unroll
-      for (int m = 0; m < MB; ++m)
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          const int j = min(j0 + wj + n * 32 + cj, a.N - 1);
-          const float* pb = (const float*)a.B + j * bj + k0 * br;
-          const float* pa = (const float*)a.A + k0 * ar;
-          int64_t row[16];
-#pragma unroll
-          for (int g = 0; g < 16; ++g) row[g] = min(i0 + wi + m * 32 + ci + (g & 3) + 8 * (g >> 2), a.M - 1) * ai;
-          floatx16 c;
-#pragma unroll
-          for (int g = 0; g < 16; ++g) c[g] = 0.0f;
-          for (int k = 0; k < have; ++k) {
-            const float bv = pb[k * br];
-#pragma unroll
-            for (int g = 0; g < 16; ++g) c[g] = fmaf(pa[row[g] + k * ar], bv, c[g]);
-          }
-          acc[m][n] = c;
-        }
+      fma_tile(a, A_ACROSS, B_ACROSS, BM, BN, THREADS, i0, j0, split, k0, have);
+      return;
     }
   }
-
   tile_end<T, MB, NB, WM * WN>(a, split, i0 + wi, j0 + wj, acc, (float*)lds);
 }
 
@@ -599,7 +593,7 @@ struct Operand16 {
 };
 
 template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int RING>
-__global__ __launch_bounds__(WM * WN * 64) void k_tile16(TileArgs a) {
+__global__ __launch_bounds__(WM * WN * 64, 2) void k_tile16(TileArgs a) {
   constexpr int WAVES = WM * WN, MB = BM / WM / 32, NB = BN / WN / 32;
   typedef Operand16<T, A_ACROSS, BM, WAVES, MB> OpA;
   typedef Operand16<T, B_ACROSS, BN, WAVES, NB> OpB;
@@ -1022,6 +1016,7 @@ struct Plan {
   int tile;                  // 128 or 256
   int splits;
   int64_t per;
+  int64_t cut;               // > 0: only these rows, in whole rounds of tiles; the others by a plan of their own
   size_t pack_a, pack_b;     // bytes of copies on 16-byte boundaries (k_tile16), 0: none
   size_t bytes;              // of workspace: the copies, then the partial sums
 };
@@ -1031,12 +1026,66 @@ bool tile16_ready(const void* p, int64_t ld) { return dense_aligned(p, 16) && ld
 size_t pack_bytes(int64_t rows, int64_t cols) { return align256((size_t)rows * ((cols + 7) / 8 * 8) * 2); }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// How a large product is cut into workgroups: 128- or 256-wide tiles, r split into `splits` parts or not.  The chip holds 256
+// workgroups with 256-wide tiles (their LDS fills a CU) and 512 with 128-wide ones, a round each.  A round costs a fixed time
+// and a time per r value; measured (us, ns per r), 2048 .. 4096 x 1024 .. 4096 with r = 512 and 2048:
+//              256-wide     128-wide, two a CU     128-wide, one a CU
+//   16 bits    12, 25       9, 18                  7, 10.4
+//   fp32       22, 150      13, 90                 13, 73
+// Split sums are written and read once more in fp32, at 5 TB/s, by one more launch (4 us).  The estimates are within 15 % of
+// what was measured: gradient of a 1536 x 512 weight over 65536 bf16 rows 256-wide / 21 parts 120 (121 measured), 128-wide / 10
+// parts 144 (135), not split 690 (390 for 4 parts).
+// A last round that is at most half full is not started (operands that are copied first aside): the rows before it are one launch, the others another (100000 x 512
+// fp32 outputs are 782 tiles, three rounds and 14 tiles).
+struct TileChoice {
+  int tile, splits;
+  int64_t cut;
+  double us;
+};
+TileChoice choose_tile(bool f32, int64_t M, int64_t N, int64_t K, bool may_cut) {
+  TileChoice best{0, 0, 0, 1e30};
+  for (int tile = 256; tile >= 128; tile /= 2) {
+    const int64_t tiles = ceil_div(M, tile) * ceil_div(N, tile);
+    for (int s = 1; s <= 64; ++s) {
+      const int64_t blocks = tiles * s;
+      if (s > 1 && (K / s < 128 || blocks > 768)) break;
+      double fixed, per_k;
+      int64_t rounds;
+      if (tile == 256) fixed = f32 ? 22 : 12, per_k = f32 ? 0.15 : 0.025, rounds = ceil_div(blocks, 256);
+      else if (blocks > 256) fixed = f32 ? 13 : 9, per_k = f32 ? 0.09 : 0.018, rounds = ceil_div(blocks, 512);
+      else fixed = f32 ? 13 : 7, per_k = f32 ? 0.073 : 0.0104, rounds = 1;
+      double us = rounds * (fixed + per_k * (double)ceil_div(K, s));
+      if (s > 1) us += 4 + 8e-6 * s * M * N / 5;
+      if (us < best.us) best = {tile, s, 0, us};
+    }
+  }
+  const int64_t nt = ceil_div(N, 256), tiles = ceil_div(M, 256) * nt, over = tiles % 256;
+  if (may_cut && tiles > 256 && over > 0 && over <= 128) {
+    const int64_t cut = (tiles - over) / nt * 256;   // whole rows of tiles
+    const double us = ceil_div(cut / 256 * nt, 256) * ((f32 ? 22 : 12) + (f32 ? 0.15 : 0.025) * K) + 4 + choose_tile(f32, M - cut, N, K, false).us;
+    if (us < best.us) best = {256, 1, cut, us};
+  }
+  return best;
+}
+
+// the product without its first `cut` rows
+Product rest_of(int type, Product q, int64_t cut) {
+  const int64_t s = (int64_t)dense_type_size(type);
+  auto on = [&](const void* p, int64_t ld) { return p ? (const void*)((const char*)p + cut * ld * s) : nullptr; };
+  q.A = on(q.A, q.a_across ? 1 : q.lda);
+  q.M -= cut;
+  q.e.out = (void*)on(q.e.out, q.e.ldo);
+  q.e.pre = (void*)on(q.e.pre, q.e.ldp);
+  q.e.residual = on(q.e.residual, q.e.ldr);
+  return q;
+}
+
 Plan plan(int type, const Product& q) {
   Plan p{};
   const bool a_across = q.a_across, b_across = q.b_across;
   const int64_t M = q.M, N = q.N, K = q.K;
   if (M == 0 || N == 0 || K == 0) return p;
-  const int V = type == DISN_F32 ? 4 : 8, KT = type == DISN_F32 ? Mma<float>::KT : KT16;
+  const int V = type == DISN_F32 ? 4 : 8, KT = type == DISN_F32 ? KT32 : KT16;
   if (!a_across && M <= 16 && K * N >= (1 << 20)) {
     p.kind = K_ROWS;
     if (!b_across) return p;
@@ -1053,15 +1102,17 @@ Plan plan(int type, const Product& q) {
     return p;
   }
   p.kind = K_TILE;
-  p.tile = ceil_div(M, 256) * ceil_div(N, 256) >= 256 ? 256 : 128;
-  const int64_t tiles = ceil_div(M, p.tile) * ceil_div(N, p.tile);
-  int64_t want = tiles >= 256 ? 1 : 512 / tiles;
-  const int64_t most = ceil_div(K, type == DISN_F32 ? 64 : 256);
-  if (want > most) want = most;
-  p.per = ceil_div(ceil_div(K, want), KT) * KT;
+  const bool pack_a = type != DISN_F32 && !tile16_ready(q.A, q.lda), pack_b = type != DISN_F32 && !tile16_ready(q.B, q.ldb);
+  const TileChoice c = choose_tile(type == DISN_F32, M, N, K, !pack_a && !pack_b);
+  p.tile = c.tile, p.splits = c.splits, p.cut = c.cut;
+  p.per = ceil_div(ceil_div(K, p.splits), KT) * KT;
   p.splits = (int)ceil_div(K, p.per);
-  if (type != DISN_F32 && !tile16_ready(q.A, q.lda)) p.pack_a = a_across ? pack_bytes(K, M) : pack_bytes(M, K);
-  if (type != DISN_F32 && !tile16_ready(q.B, q.ldb)) p.pack_b = b_across ? pack_bytes(K, N) : pack_bytes(N, K);
+  if (p.cut) {   // the two parts run one after the other
+    p.bytes = plan(type, rest_of(type, q, p.cut)).bytes;
+    return p;
+  }
+  if (pack_a) p.pack_a = a_across ? pack_bytes(K, M) : pack_bytes(M, K);
+  if (pack_b) p.pack_b = b_across ? pack_bytes(K, N) : pack_bytes(N, K);
   p.bytes = p.pack_a + p.pack_b + (p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0);
   return p;
 }
@@ -1070,9 +1121,11 @@ template <typename T>
 int launch_finish(DisnCtx* ctx, const float* part, int nparts, int64_t M, int64_t N, const Epilogue& e, hipStream_t stream) {
   if (M == 0 || N == 0) return DISN_OK;
   const int64_t vecs = M * ceil_div(N, Vec<T>::N);
-  // below 64 workgroups' worth of results the parts are shared
+  // with less than 64 / 256 workgroups' worth of results the parts are shared
   if (nparts >= 16 && vecs <= 1 << 14)
     k_finish<T, 16><<<(unsigned)ceil_div(vecs, 16), 256, 0, stream>>>(part, nparts, M, (int)N, e);
+  else if (nparts >= 8 && vecs <= 1 << 16)
+    k_finish<T, 4><<<(unsigned)ceil_div(vecs, 64), 256, 0, stream>>>(part, nparts, M, (int)N, e);
   else
     k_finish<T, 1><<<(unsigned)(ceil_div(vecs, 256) < 8192 ? ceil_div(vecs, 256) : 8192), 256, 0, stream>>>(part, nparts, M, (int)N, e);
   DISN_HIP(ctx, hipGetLastError());
@@ -1085,7 +1138,7 @@ int launch_tile(DisnCtx* ctx, const TileArgs& a, hipStream_t stream) {
   const void* kernel;
   int bytes;
   if constexpr (sizeof(T) == 4) {
-    kernel = (const void*)k_tile<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN>;
+    kernel = (const void*)k_tile32<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN>;
     bytes = 2 * (Operand<T, A_ACROSS, BM, THREADS>::BYTES + Operand<T, B_ACROSS, BN, THREADS>::BYTES);
   } else {
     kernel = (const void*)k_tile16<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN, RING>;
@@ -1138,7 +1191,13 @@ int64_t small_blocks(const SmallArgs& s) { return (int64_t)s.mt * ceil_div(s.nt,
 
 // one product by its plan; ws: plan.bytes of workspace
 template <typename T>
-int run_product(DisnCtx* ctx, Product q, const Plan& p, char* ws, hipStream_t stream) {
+int run_product(DisnCtx* ctx, Product q, Plan p, char* ws, hipStream_t stream) {
+  if (p.cut) {
+    const Product rest = rest_of(sizeof(T) == 4 ? DISN_F32 : DISN_BF16, q, p.cut);
+    DISN_TRY(run_product<T>(ctx, rest, plan(sizeof(T) == 4 ? DISN_F32 : DISN_BF16, rest), ws, stream));
+    q.M = p.cut;
+    p.cut = 0;
+  }
   float* part = (float*)(ws + p.pack_a + p.pack_b);
   if constexpr (sizeof(T) == 2) {
     if (p.pack_a) DISN_TRY(launch_pack<T>(ctx, &q.A, &q.lda, q.a_across ? q.K : q.M, q.a_across ? q.M : q.K, ws, stream));
@@ -1250,10 +1309,10 @@ GradPlan plan_backward(const DisnLinearGrad* a) {
   while (g.gate_lanes < 64 && g.gate_lanes * V < a->n) g.gate_lanes *= 2;
   g.gate_groups = (int)ceil_div(a->n, g.gate_lanes * V);
   if (g.gate_groups < 1) g.gate_groups = 1;
-  // row blocks: about 1024 workgroups, at least 8 rows a thread
+  // row blocks: about 1024 workgroups, at least 4 rows a thread
   const int64_t lines = 256 / g.gate_lanes;
   int64_t blocks = ceil_div(1024, g.gate_groups);
-  if (blocks > ceil_div(a->m, lines * 8)) blocks = ceil_div(a->m, lines * 8);
+  if (blocks > ceil_div(a->m, lines * 4)) blocks = ceil_div(a->m, lines * 4);
   if (blocks < 1) blocks = 1;
   g.gate_rows = ceil_div(a->m, blocks);
   g.gate_blocks = a->m ? ceil_div(a->m, g.gate_rows) : 0;
