@@ -593,7 +593,7 @@ struct Operand16 {
 };
 
 template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int RING>
-__global__ __launch_bounds__(WM * WN * 64, 2) void k_tile16(TileArgs a) {
+__global__ __launch_bounds__(WM * WN * 64, BM == 128 ? 3 : 2) void k_tile16(TileArgs a) {
   constexpr int WAVES = WM * WN, MB = BM / WM / 32, NB = BN / WN / 32;
   typedef Operand16<T, A_ACROSS, BM, WAVES, MB> OpA;
   typedef Operand16<T, B_ACROSS, BN, WAVES, NB> OpB;
@@ -1026,22 +1026,29 @@ bool tile16_ready(const void* p, int64_t ld) { return dense_aligned(p, 16) && ld
 size_t pack_bytes(int64_t rows, int64_t cols) { return align256((size_t)rows * ((cols + 7) / 8 * 8) * 2); }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// How a large product is cut into workgroups: 128- or 256-wide tiles, r split into `splits` parts or not.  The chip holds 256
-// workgroups with 256-wide tiles (their LDS fills a CU) and 512 with 128-wide ones, a round each.  A round costs a fixed time
-// and a time per r value; measured (us, ns per r), 2048 .. 4096 x 1024 .. 4096 with r = 512 and 2048:
-//              256-wide     128-wide, two a CU     128-wide, one a CU
-//   16 bits    12, 25       9, 18                  7, 10.4
-//   fp32       22, 150      13, 90                 13, 73
+// How a large product is cut into workgroups: 128- or 256-wide tiles, r split into `splits` parts or not.  A CU holds one
+// workgroup with 256-wide tiles (its LDS), two with 128-wide ones, or three of those with a ring of three stages.  A round of
+// them costs a fixed time and a time per r value; measured (us, ns per r), 2048 .. 65536 x 512 .. 4096, r = 128 .. 2048:
+//              256-wide     128-wide: one a CU    two         three
+//   16 bits    12, 26                 7, 10.4     9, 17       7.5, 24
+//   fp32       22, 150                13, 73      13, 90
 // Split sums are written and read once more in fp32, at 5 TB/s, by one more launch (4 us).  The estimates are within 15 % of
-// what was measured: gradient of a 1536 x 512 weight over 65536 bf16 rows 256-wide / 21 parts 120 (121 measured), 128-wide / 10
-// parts 144 (135), not split 690 (390 for 4 parts).
-// A last round that is at most half full is not started (operands that are copied first aside): the rows before it are one launch, the others another (100000 x 512
-// fp32 outputs are 782 tiles, three rounds and 14 tiles).
+// what was measured: gradient of a 1536 x 512 weight over 65536 bf16 rows 256-wide / 21 parts 123 (121 measured), 128-wide / 10
+// parts 137 (135); 65536 x 512 outputs with r = 128 256-wide 31 (32), 128-wide 29 (28), r = 1536 103 (113), 118 (120).
+// A last round that is at most half full is not started (operands that are copied first aside): the rows before it are one
+// launch, the others another (100000 x 512 fp32 outputs are 782 tiles, three rounds and 14 tiles).
 struct TileChoice {
   int tile, splits;
   int64_t cut;
   double us;
 };
+double tile_rounds_us(bool f32, int tile, int64_t blocks, double r) {
+  if (tile == 256) return (double)ceil_div(blocks, 256) * (f32 ? 22 + 0.15 * r : 12 + 0.026 * r);
+  const double one = f32 ? 13 + 0.073 * r : 7 + 0.0104 * r, two = f32 ? 13 + 0.09 * r : 9 + 0.017 * r;
+  const int64_t full = f32 ? 512 : 768, last = blocks > 512 ? blocks % full : blocks;
+  const double three = 7.5 + 0.024 * r, whole = blocks > 512 ? (double)(blocks / full) * (f32 ? two : three) : 0;
+  return whole + (last == 0 ? 0 : last <= 256 ? one : last <= 512 ? two : three);
+}
 TileChoice choose_tile(bool f32, int64_t M, int64_t N, int64_t K, bool may_cut) {
   TileChoice best{0, 0, 0, 1e30};
   for (int tile = 256; tile >= 128; tile /= 2) {
@@ -1049,12 +1056,7 @@ TileChoice choose_tile(bool f32, int64_t M, int64_t N, int64_t K, bool may_cut) 
     for (int s = 1; s <= 64; ++s) {
       const int64_t blocks = tiles * s;
       if (s > 1 && (K / s < 128 || blocks > 768)) break;
-      double fixed, per_k;
-      int64_t rounds;
-      if (tile == 256) fixed = f32 ? 22 : 12, per_k = f32 ? 0.15 : 0.025, rounds = ceil_div(blocks, 256);
-      else if (blocks > 256) fixed = f32 ? 13 : 9, per_k = f32 ? 0.09 : 0.018, rounds = ceil_div(blocks, 512);
-      else fixed = f32 ? 13 : 7, per_k = f32 ? 0.073 : 0.0104, rounds = 1;
-      double us = rounds * (fixed + per_k * (double)ceil_div(K, s));
+      double us = tile_rounds_us(f32, tile, blocks, (double)ceil_div(K, s));
       if (s > 1) us += 4 + 8e-6 * s * M * N / 5;
       if (us < best.us) best = {tile, s, 0, us};
     }
@@ -1062,7 +1064,7 @@ TileChoice choose_tile(bool f32, int64_t M, int64_t N, int64_t K, bool may_cut) 
   const int64_t nt = ceil_div(N, 256), tiles = ceil_div(M, 256) * nt, over = tiles % 256;
   if (may_cut && tiles > 256 && over > 0 && over <= 128) {
     const int64_t cut = (tiles - over) / nt * 256;   // whole rows of tiles
-    const double us = ceil_div(cut / 256 * nt, 256) * ((f32 ? 22 : 12) + (f32 ? 0.15 : 0.025) * K) + 4 + choose_tile(f32, M - cut, N, K, false).us;
+    const double us = tile_rounds_us(f32, 256, cut / 256 * nt, (double)K) + 4 + choose_tile(f32, M - cut, N, K, false).us;
     if (us < best.us) best = {256, 1, cut, us};
   }
   return best;
@@ -1157,8 +1159,10 @@ int launch_tile(DisnCtx* ctx, const TileArgs& a, hipStream_t stream) {
 }
 template <typename T, bool A_ACROSS, bool B_ACROSS>
 int launch_tile(DisnCtx* ctx, int tile, const TileArgs& a, hipStream_t stream) {
-  return tile == 256 ? launch_tile<T, A_ACROSS, B_ACROSS, 256, 256, 2, 4, 4>(ctx, a, stream)
-                     : launch_tile<T, A_ACROSS, B_ACROSS, 128, 128, 2, 2, 4>(ctx, a, stream);
+  if (tile == 256) return launch_tile<T, A_ACROSS, B_ACROSS, 256, 256, 2, 4, 4>(ctx, a, stream);
+  if constexpr (sizeof(T) == 2)   // 48 KB of LDS: three a CU
+    if ((int64_t)a.mt * a.nt * a.splits > 512) return launch_tile<T, A_ACROSS, B_ACROSS, 128, 128, 2, 2, 3>(ctx, a, stream);
+  return launch_tile<T, A_ACROSS, B_ACROSS, 128, 128, 2, 2, 4>(ctx, a, stream);
 }
 // a copy of rows x cols values at dst, 16-byte boundaries; *p, *ld become it
 template <typename T>
