@@ -64,6 +64,7 @@ class Context:
         if rc != 0:
             raise DisnError("disn_create(%s) failed with %d" % (self.device, rc))
         self._h = h
+        self._index = self.device.index or 0
         self._mc_counts = None
         self.auto_decoder = True       # decoder arithmetic chosen by measurement at the first evaluation after set_weights
         self._tuned = False
@@ -228,7 +229,7 @@ class Context:
     # A small call takes the GPU about 4 us, so the wrapper's own time counts: cheap checks, one struct, no copies where none
     # are needed.
     def _tensor(self, t, what, dtype):
-        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != self.device or t.layout is not torch.strided:
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != self._index or t.layout is not torch.strided:
             raise DisnError("%s must be a %s tensor on %s" % (what, dtype, self.device))
 
     def _rows(self, t, what, dtype, shape, copy=True):
@@ -237,12 +238,14 @@ class Context:
         if t.shape != shape:
             raise DisnError("%s has shape %s, expected %s" % (what, tuple(t.shape), tuple(shape)))
         c = shape[-1]
+        if t.is_contiguous():
+            return t, (t.data_ptr(), shape[0] if len(shape) == 2 else t.numel() // c if c else 0, c, c, t.element_size())
         if len(shape) == 2:
             n, (ld, unit) = shape[0], t.stride()
         else:
-            n = t.numel() // c if c else 0
+            n = t.numel() // c
             unit, ld = t.stride(-1), c
-            if len(shape) > 2 and not t.is_contiguous():
+            if len(shape) > 2:
                 try:
                     ld = t.view(n, c).stride(0)
                 except RuntimeError:
@@ -265,22 +268,22 @@ class Context:
         return t, t.data_ptr()
 
     def _weight(self, w, what, dtype):
-        """[k][n] weights in either order of memory -> (tensor, w_nk, address, row distance)"""
+        """[k][n] weights in either order of memory -> (tensor, k, n, w_nk, address, row distance)"""
         self._tensor(w, what, dtype)
         if w.dim() != 2:
             raise DisnError("%s must be a [k, n] matrix" % what)
         k, n = w.shape
         s0, s1 = w.stride()
         if (s1 == 1 or n <= 1) and (s0 >= n or k <= 1):
-            return w, 0, w.data_ptr(), n if k <= 1 else s0
+            return w, k, n, 0, w.data_ptr(), n if k <= 1 else s0
         if (s0 == 1 or k <= 1) and s1 >= k:
-            return w, 1, w.data_ptr(), k if n <= 1 else s1
+            return w, k, n, 1, w.data_ptr(), k if n <= 1 else s1
         w = w.contiguous()
-        return w, 0, w.data_ptr(), n
+        return w, k, n, 0, w.data_ptr(), n
 
     def _elsewhere(self):
         """whether another device than the context's is the current one"""
-        return torch.cuda.current_device() != self.device.index
+        return torch._C._cuda_getDevice() != self._index
 
     def _run(self, query, call, name, args, like):
         """a call with the workspace it asks for, on the current stream of the context's device"""
@@ -292,7 +295,7 @@ class Context:
                 self._check(rc, name)
             if n.value:
                 ws = like.new_empty(n.value, dtype=torch.uint8)
-        stream = torch._C._cuda_getCurrentRawStream(self.device.index)   # current_stream().cuda_stream without the object
+        stream = torch._C._cuda_getCurrentRawStream(self._index)   # current_stream().cuda_stream without the object
         rc = call(self._h, ref, stream) if query is None else call(self._h, ref, ws.data_ptr() if ws is not None else None, n.value, stream)
         if rc:
             self._check(rc, name)
@@ -313,12 +316,14 @@ class Context:
         dtype = self._type(x, "linear: x")
         if act not in ACTS:
             raise DisnError("linear: unknown act %r (have %s)" % (act, ", ".join(ACTS)))
-        w, w_nk, wp, ldw = self._weight(w, "linear: w", dtype)
-        k, n = w.shape
-        lead = x.shape[:-1]
-        shape = lead + (n,)
-        x, xm = self._rows(x, "linear: x", dtype, lead + (k,))
-        m = xm[1] if k else lead.numel()
+        w, k, n, w_nk, wp, ldw = self._weight(w, "linear: w", dtype)
+        if x.dim() == 2:
+            m = x.shape[0]
+            shape, xshape = (m, n), (m, k)
+        else:
+            lead = x.shape[:-1]
+            m, shape, xshape = lead.numel(), lead + (n,), lead + (k,)
+        x, xm = self._rows(x, "linear: x", dtype, xshape)
         bias, bp = self._vec(bias, "linear: bias", dtype, n)
         rm = (None, 0, 0, 0)
         if residual is not None:
@@ -357,9 +362,8 @@ class Context:
         lead, n = dy.shape[:-1], dy.shape[-1]
         w_nk, wp, ldw, k = 0, None, 0, 0
         if w is not None:
-            w, w_nk, wp, ldw = self._weight(w, "linear_backward: w", dtype)
-            k = w.shape[0]
-            if w.shape[1] != n:
+            w, k, wn, w_nk, wp, ldw = self._weight(w, "linear_backward: w", dtype)
+            if wn != n:
                 raise DisnError("linear_backward: w has shape %s, dy %s" % (tuple(w.shape), tuple(dy.shape)))
         elif x is not None:
             k = x.shape[-1]

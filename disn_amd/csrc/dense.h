@@ -80,8 +80,15 @@ __global__ __launch_bounds__(256) void k_sum_partials(const float* __restrict__ 
   const int64_t col = (int64_t)blockIdx.x * 16 + c;
   float s = 0.0f;
   if (col < ncols) {
-#pragma unroll 4
-    for (int p = g; p < nparts; p += 16) s += part[(size_t)p * ncols + col];
+    int p = g;
+    for (; p + 15 * 16 < nparts; p += 16 * 16) {   // sixteen loads under way
+      float v[16];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) v[u] = part[(size_t)(p + u * 16) * ncols + col];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) s += v[u];
+    }
+    for (; p < nparts; p += 16) s += part[(size_t)p * ncols + col];
   }
   lds[g][c] = s;
   __syncthreads();

@@ -13,6 +13,7 @@
 #include "dense.h"
 
 #include <atomic>
+#include <type_traits>
 
 namespace {
 
@@ -292,7 +293,7 @@ __device__ __forceinline__ floatx16 mfma(shortx8 a, shortx8 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-template <typename T, bool ACROSS, int ROWS, int THREADS>
+template <typename T, bool ACROSS, int ROWS, int THREADS, int DEPTH>
 struct Operand {
   static constexpr int KT = KT32, P = PLANES, V = Vec<T>::N;
   static constexpr int PER_LINE = (ACROSS ? ROWS : KT) / V;    // 16-byte pieces in a contiguous run
@@ -307,7 +308,7 @@ struct Operand {
   int64_t ld;
   int left;          // i values in the tile
   int first;         // the stage's first value in its row
-  Vec<T> reg[Q];
+  Vec<T> reg[DEPTH][Q];   // stages under way
 
   __device__ __forceinline__ void init(const T* p, int64_t ld_, int i0, int n_i, int64_t k0) {
     ld = ld_;
@@ -323,34 +324,32 @@ struct Operand {
         ptr[q] = p + (int64_t)(i0 + (line < left ? line : left - 1)) * ld + k0 + c;
     }
   }
-  // the next stage, of which `have` (>= 1) r values exist; zeros behind them
-  __device__ __forceinline__ void fetch(int have) {
-    if (have >= KT && (!ACROSS || left >= ROWS)) {
+  // whether whole stages need no ends to be cut
+  __device__ __forceinline__ bool inside() const { return !ACROSS || left >= ROWS; }
+  // the next stage, of which `have` (>= 1) r values exist, into reg[slot]; zeros behind them
+  template <bool WHOLE>
+  __device__ __forceinline__ void fetch(int slot, int have) {
 #pragma unroll
-      for (int q = 0; q < Q; ++q) reg[q] = load_vec(ptr[q]);
-    } else {
-#pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        const int t = threadIdx.x + q * THREADS, line = t / PER_LINE, c = t % PER_LINE * V;
-        if (ACROSS) {
-          reg[q] = load_vec(ptr[q] - (line < have ? 0 : line * ld), line < have ? (c < left ? left - c : left) : 0, first + (c < left ? c : 0));
-        } else {
-          reg[q] = load_vec(ptr[q] - (c < have ? 0 : c), have - c, first + c);
-        }
-      }
+    for (int q = 0; q < Q; ++q) {
+      const int t = threadIdx.x + q * THREADS, line = t / PER_LINE, c = t % PER_LINE * V;
+      if (WHOLE)
+        reg[slot][q] = load_vec(ptr[q]);
+      else if (ACROSS)
+        reg[slot][q] = load_vec(ptr[q] - (line < have ? 0 : line * ld), line < have ? (c < left ? left - c : left) : 0, first + (c < left ? c : 0));
+      else
+        reg[slot][q] = load_vec(ptr[q] - (c < have ? 0 : c), have - c, first + c);
+      ptr[q] += ACROSS ? KT * ld : KT;
     }
-#pragma unroll
-    for (int q = 0; q < Q; ++q) ptr[q] += ACROSS ? KT * ld : KT;
     if (!ACROSS) first += KT;
   }
-  __device__ __forceinline__ void store(char* lds) const {
+  __device__ __forceinline__ void store(char* lds, int slot) const {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int t = threadIdx.x + q * THREADS, line = t / PER_LINE, c = t % PER_LINE * V;
       char* dst = lds + (ACROSS ? line * LINE + c * 2 : (c >> 3) * BLOCK + line * 16 + (c & 7) * 2);
       float rest[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) rest[i] = reg[q].v[i];
+      for (int i = 0; i < 4; ++i) rest[i] = reg[slot][q].v[i];
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         bf16_t term[4];
@@ -410,11 +409,11 @@ __device__ __forceinline__ void fma_tile(const TileArgs& a, bool a_across, bool 
   }
 }
 
-template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN>
+template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int DEPTH>
 __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile32(TileArgs a) {
   constexpr int THREADS = WM * WN * 64, MB = BM / WM / 32, NB = BN / WN / 32, KT = KT32, P = PLANES;
-  typedef Operand<T, A_ACROSS, BM, THREADS> OpA;
-  typedef Operand<T, B_ACROSS, BN, THREADS> OpB;
+  typedef Operand<T, A_ACROSS, BM, THREADS, DEPTH> OpA;
+  typedef Operand<T, B_ACROSS, BN, THREADS, DEPTH> OpB;
   constexpr int BUF = OpA::BYTES + OpB::BYTES;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const TilePlace at = tile_place(a, BM, BN);
@@ -436,26 +435,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile32(TileArgs a) {
   OpB B;
   A.init((const T*)a.A, a.lda, i0, a.M, k0);
   B.init((const T*)a.B, a.ldb, j0, a.N, k0);
-  A.fetch(have);
-  B.fetch(have);
-  A.store(lds);
-  B.store(lds + OpA::BYTES);
-  if (stages > 1) {
-    A.fetch(have - KT);
-    B.fetch(have - KT);
-  }
-  for (int s = 0; s < stages; ++s) {
-    __syncthreads();   // stage s is in LDS for everyone, stage s - 1 has been read by everyone
-    const char* cur = lds + (s & 1) * BUF;
-    char* nxt = lds + (~s & 1) * BUF;
-    if (s + 1 < stages) {
-      A.store(nxt);
-      B.store(nxt + OpA::BYTES);
-    }
-    if (s + 2 < stages) {
-      A.fetch(have - (s + 2) * KT);
-      B.fetch(have - (s + 2) * KT);
-    }
+  auto multiply = [&](int buffer) {
+    const char* cur = lds + buffer * BUF;
 #pragma unroll
     for (int q = 0; q < KT / 16; ++q) {
       shortx8 b[NB][P];
@@ -479,7 +460,41 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile32(TileArgs a) {
         }
       }
     }
-  }
+  };
+  // stage s is multiplied from one buffer while s + 1 goes from its registers into the other and s + 1 + DEPTH is fetched
+  auto step = [&](int s, int u, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    __syncthreads();   // stage s is in LDS for everyone, stage s - 1 has been read by everyone
+    const int buffer = DEPTH == 2 ? u : s & 1, slot = (u + 1) % DEPTH;
+    if (WHOLE || s + 1 < stages) {
+      A.store(lds + (1 - buffer) * BUF, slot);
+      B.store(lds + (1 - buffer) * BUF + OpA::BYTES, slot);
+    }
+    if (WHOLE || s + 1 + DEPTH < stages) {
+      A.template fetch<WHOLE>(slot, have - (s + 1 + DEPTH) * KT);
+      B.template fetch<WHOLE>(slot, have - (s + 1 + DEPTH) * KT);
+    }
+    multiply(buffer);
+  };
+  A.template fetch<false>(0, have);
+  B.template fetch<false>(0, have);
+  A.store(lds, 0);
+  B.store(lds + OpA::BYTES, 0);
+#pragma unroll
+  for (int d = 1; d <= DEPTH; ++d)
+    if (d < stages) {
+      A.template fetch<false>(d % DEPTH, have - d * KT);
+      B.template fetch<false>(d % DEPTH, have - d * KT);
+    }
+  const int whole = A.inside() && B.inside() ? have / KT : 0;
+  int s = 0;
+  for (; s + 2 * DEPTH < whole; s += DEPTH)
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u) step(s + u, u, std::true_type());
+  for (; s < stages; s += DEPTH)
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u)
+      if (s + u < stages) step(s + u, u, std::false_type());
 
   static_assert(32 * tile_stride(NB) * 4 * WM * WN <= 2 * BUF, "the turned tiles fit into the stage buffers");
   {
@@ -1140,8 +1155,9 @@ int launch_tile(DisnCtx* ctx, const TileArgs& a, hipStream_t stream) {
   const void* kernel;
   int bytes;
   if constexpr (sizeof(T) == 4) {
-    kernel = (const void*)k_tile32<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN>;
-    bytes = 2 * (Operand<T, A_ACROSS, BM, THREADS>::BYTES + Operand<T, B_ACROSS, BN, THREADS>::BYTES);
+    constexpr int DEPTH = BM == 128 ? 2 : 1;   // a stage of a 128-wide tile is over before the next has come
+    kernel = (const void*)k_tile32<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN, DEPTH>;
+    bytes = 2 * (Operand<T, A_ACROSS, BM, THREADS, DEPTH>::BYTES + Operand<T, B_ACROSS, BN, THREADS, DEPTH>::BYTES);
   } else {
     kernel = (const void*)k_tile16<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN, RING>;
     bytes = RING * (BM + BN) * KT16 * 2;

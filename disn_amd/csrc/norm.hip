@@ -52,16 +52,20 @@ __device__ __forceinline__ void widen(const Vec<T> (&in)[E / Vec<T>::N], float (
   for (int i = 0; i < E; ++i) out[i] = (float)in[i / Vec<T>::N].v[i % Vec<T>::N];
 }
 
-template <typename T, int G, int E>
+// EVEN: rows of whole pieces, which need no ends to be cut
+template <typename T, int G, int E, bool EVEN>
 __device__ __forceinline__ void load_row(const T* row, int t, int d, Vec<T> (&out)[E / Vec<T>::N]) {
 #pragma unroll
   for (int p = 0; p < E / Vec<T>::N; ++p) {
     const int c = piece_col<T, G>(t, p);
-    out[p] = load_vec(row + (c < d ? c : 0), c < d ? d - c : 0, c);
+    if (EVEN)
+      out[p] = c < d ? load_vec(row + c) : Vec<T>{};
+    else
+      out[p] = load_vec(row + (c < d ? c : 0), c < d ? d - c : 0, c);
   }
 }
 
-template <typename T, int G, int E>
+template <typename T, int G, int E, bool EVEN>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm(NormArgs a) {
   constexpr int N = Vec<T>::N, P = E / N, B = G < 256 ? 256 : G;
   __shared__ float lds[2][16];
@@ -81,7 +85,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm(NormArgs a) {
   const float inv = 1.0f / (float)d;
   for (int64_t row = (int64_t)blockIdx.x * (B / G) + threadIdx.x / G; row < a.rows; row += (int64_t)gridDim.x * (B / G)) {
     Vec<T> xv[P];
-    load_row<T, G, E>((const T*)a.x + row * a.ldx, t, d, xv);
+    load_row<T, G, E, EVEN>((const T*)a.x + row * a.ldx, t, d, xv);
     float x[E];
     widen<T, E>(xv, x);
     float s = 0.0f;
@@ -110,12 +114,12 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm(NormArgs a) {
       Vec<T> o;
 #pragma unroll
       for (int i = 0; i < N; ++i) o.v[i] = (T)fmaf(x[p * N + i] * rstd, w[p * N + i], b[p * N + i]);
-      store_vec(y + c, o, d - c);
+      store_vec(y + c, o, EVEN ? N : d - c);
     }
   }
 }
 
-template <typename T, int G, int E>
+template <typename T, int G, int E, bool EVEN>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm_backward(NormArgs a) {
   constexpr int N = Vec<T>::N, P = E / N, B = G < 256 ? 256 : G;
   __shared__ float lds[2][16];
@@ -133,9 +137,9 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm_backward(NormA
   const float inv = 1.0f / (float)d;
   for (int64_t row = (int64_t)blockIdx.x * (B / G) + threadIdx.x / G; row < a.rows; row += (int64_t)gridDim.x * (B / G)) {
     Vec<T> xv[P], gv[P], rv[P];
-    load_row<T, G, E>((const T*)a.x + row * a.ldx, t, d, xv);
-    load_row<T, G, E>((const T*)a.dy + row * a.lddy, t, d, gv);
-    if (a.y && a.residual) load_row<T, G, E>((const T*)a.residual + row * a.ldr, t, d, rv);
+    load_row<T, G, E, EVEN>((const T*)a.x + row * a.ldx, t, d, xv);
+    load_row<T, G, E, EVEN>((const T*)a.dy + row * a.lddy, t, d, gv);
+    if (a.y && a.residual) load_row<T, G, E, EVEN>((const T*)a.residual + row * a.ldr, t, d, rv);
     const float mean = a.mean_in[row], rstd = a.rstd_in[row];
     float h[E], g[E], s1 = 0.0f, s2 = 0.0f;
     widen<T, E>(xv, h);
@@ -167,7 +171,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm_backward(NormA
         if (a.residual) v += (float)rv[p].v[i];
         o.v[i] = (T)v;
       }
-      store_vec(dx + c, o, d - c);
+      store_vec(dx + c, o, EVEN ? N : d - c);
     }
   }
   if (!a.dweight && !a.dbias) return;
@@ -233,10 +237,11 @@ int64_t norm_backward_grid(const NormShape& s, int64_t rows) {
 template <typename T, int G, int E>
 void launch_norm(bool backward, const NormArgs& a, int64_t grid, hipStream_t stream) {
   constexpr int B = G < 256 ? 256 : G;
-  if (backward)
-    k_layer_norm_backward<T, G, E><<<(unsigned)grid, B, 0, stream>>>(a);
-  else
-    k_layer_norm<T, G, E><<<(unsigned)grid, B, 0, stream>>>(a);
+  const bool even = a.d % Vec<T>::N == 0;
+  if (backward && even) k_layer_norm_backward<T, G, E, true><<<(unsigned)grid, B, 0, stream>>>(a);
+  else if (backward) k_layer_norm_backward<T, G, E, false><<<(unsigned)grid, B, 0, stream>>>(a);
+  else if (even) k_layer_norm<T, G, E, true><<<(unsigned)grid, B, 0, stream>>>(a);
+  else k_layer_norm<T, G, E, false><<<(unsigned)grid, B, 0, stream>>>(a);
 }
 template <typename T>
 void launch_norm(const NormShape& s, bool backward, const NormArgs& a, int64_t grid, hipStream_t stream) {

@@ -9,7 +9,7 @@ from disn_amd import api
 @pytest.fixture
 def ctx(monkeypatch):
     c = api.Context.__new__(api.Context)
-    c.device = torch.device("cpu")
+    c.device, c._index = torch.device("cpu"), -1
     c.lib = type("NoLibrary", (), {"__getattr__": lambda self, name: name})()
     monkeypatch.setattr(api.Context, "_elsewhere", lambda self: False)
     monkeypatch.setattr(api.Context, "_run", lambda *a: pytest.fail("the call should have been refused"))
@@ -39,12 +39,12 @@ def test_rows(ctx):
 def test_weights(ctx):
     w = torch.arange(60.0).reshape(5, 12)
     f = torch.float32
-    assert ctx._weight(w, "w", f)[1:] == (0, w.data_ptr(), 12)
-    assert ctx._weight(w[:, 2:7], "w", f)[1:] == (0, w.data_ptr() + 8, 12)
-    assert ctx._weight(w.t(), "w", f)[1:] == (1, w.data_ptr(), 12)
-    assert ctx._weight(w[1:3, 1:9].t(), "w", f)[1:] == (1, w[1:, 1:].data_ptr(), 12)
+    assert ctx._weight(w, "w", f)[1:] == (5, 12, 0, w.data_ptr(), 12)
+    assert ctx._weight(w[:, 2:7], "w", f)[1:] == (5, 5, 0, w.data_ptr() + 8, 12)
+    assert ctx._weight(w.t(), "w", f)[1:] == (12, 5, 1, w.data_ptr(), 12)
+    assert ctx._weight(w[1:3, 1:9].t(), "w", f)[1:] == (8, 2, 1, w[1:, 1:].data_ptr(), 12)
     for view in (w[:, ::2], w[:1, :1].expand(5, 12), w[:1].expand(5, 12)):
-        copy, nk, at, ld = ctx._weight(view, "w", f)
+        copy, _, _, nk, at, ld = ctx._weight(view, "w", f)
         assert nk == 0 and ld == view.shape[1] and torch.equal(copy, view) and at == copy.data_ptr()
 
 
