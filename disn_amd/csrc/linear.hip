@@ -461,32 +461,46 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile32(TileArgs a) {
       }
     }
   };
+  const int whole = A.inside() && B.inside() ? have / KT : 0;   // stages that need no ends to be cut
+  auto fetch = [&](int slot, int stage) {
+    if (stage < whole) {
+      A.template fetch<true>(slot, KT);
+      B.template fetch<true>(slot, KT);
+    } else if (stage < stages) {
+      A.template fetch<false>(slot, have - stage * KT);
+      B.template fetch<false>(slot, have - stage * KT);
+    }
+  };
   // stage s is multiplied from one buffer while s + 1 goes from its registers into the other and s + 1 + DEPTH is fetched
   auto step = [&](int s, int u, auto whole) {
     constexpr bool WHOLE = decltype(whole)::value;
     __syncthreads();   // stage s is in LDS for everyone, stage s - 1 has been read by everyone
     const int buffer = DEPTH == 2 ? u : s & 1, slot = (u + 1) % DEPTH;
+    multiply(buffer);
     if (WHOLE || s + 1 < stages) {
       A.store(lds + (1 - buffer) * BUF, slot);
       B.store(lds + (1 - buffer) * BUF + OpA::BYTES, slot);
     }
-    if (WHOLE || s + 1 + DEPTH < stages) {
-      A.template fetch<WHOLE>(slot, have - (s + 1 + DEPTH) * KT);
-      B.template fetch<WHOLE>(slot, have - (s + 1 + DEPTH) * KT);
+    if (WHOLE) {
+      A.template fetch<true>(slot, KT);
+      B.template fetch<true>(slot, KT);
+    } else {
+      fetch(slot, s + 1 + DEPTH);
     }
-    multiply(buffer);
+    if (WHOLE) {
+      // the cutting of stage s + 1 runs between the matrix instructions of stage s
+#pragma unroll
+      for (int i = 0; i < MB * NB * 6; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 6, 0);
+      }
+    }
   };
-  A.template fetch<false>(0, have);
-  B.template fetch<false>(0, have);
+  fetch(0, 0);
   A.store(lds, 0);
   B.store(lds + OpA::BYTES, 0);
 #pragma unroll
-  for (int d = 1; d <= DEPTH; ++d)
-    if (d < stages) {
-      A.template fetch<false>(d % DEPTH, have - d * KT);
-      B.template fetch<false>(d % DEPTH, have - d * KT);
-    }
-  const int whole = A.inside() && B.inside() ? have / KT : 0;
+  for (int d = 1; d <= DEPTH; ++d) fetch(d % DEPTH, d);
   int s = 0;
   for (; s + 2 * DEPTH < whole; s += DEPTH)
 #pragma unroll
