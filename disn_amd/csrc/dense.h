@@ -20,6 +20,24 @@ __device__ __forceinline__ Vec<T> load_vec(const T* p) {
   __builtin_memcpy(&r, p, 16);
   return r;
 }
+// rounds N values to T, two at a time (one conversion instruction each)
+template <typename T, int N>
+__device__ __forceinline__ void narrow(const float* z, T* out) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = z[i];
+  } else {
+    typedef __attribute__((ext_vector_type(2))) float float2v;
+    typedef __attribute__((ext_vector_type(2))) T pair;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const pair p = __builtin_convertvector((float2v){z[i], z[i + 1]}, pair);
+      out[i] = p[0];
+      out[i + 1] = p[1];
+    }
+  }
+}
+
 // The first n values at p (n >= N: all, n <= 0: none), zeros behind them; nothing outside the row is read.  before: how
 // many values of the row lie in front of p; with N - n of them the piece is read from so much further in front and shifted.
 // (No sequence of single loads beside the wide one: hipcc merges the two into three narrow loads for every lane.)

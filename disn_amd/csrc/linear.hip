@@ -116,8 +116,7 @@ __device__ __forceinline__ void finish_vec(const Epilogue& e, int64_t row, int c
   }
   Vec<T> o;
   if (e.pre) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) o.v[i] = (T)z[i];
+    narrow<T, N>(z, o.v);
     store_vec((T*)e.pre + row * e.ldp + col, o, n);
   }
   activate_all(z, e.act);
@@ -125,8 +124,7 @@ __device__ __forceinline__ void finish_vec(const Epilogue& e, int64_t row, int c
 #pragma unroll
     for (int i = 0; i < N; ++i) z[i] += (float)residual.v[i];
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i) o.v[i] = (T)z[i];
+  narrow<T, N>(z, o.v);
   store_vec((T*)e.out + row * e.ldo + col, o, n);
 }
 template <typename T>
@@ -219,12 +217,12 @@ __device__ __forceinline__ void tile_end(const TileArgs& a, int split, int iw, i
     return;
   }
   // Memory operations of a wave end in order, so a wait for a load is a wait for the stores before it: the bias is read
-  // once, the residual two pieces ahead.  The loops stay loops: unrolled, they are 80 KB of code.
+  // once, the residual of two pieces before the two in front of them are stored.  The loops stay loops: unrolled, they are 80 KB of code.
   constexpr int W = NB * 32, V = Vec<T>::N, STRIDE = tile_stride(NB), Q = 32 * W / V / 64, STEP = 64 / (W / V);
   const int c = lane % (W / V) * V, j = jw + c, n_j = a.N - j, r0 = lane / (W / V);
   const Vec<T> bias = bias_vec<T>(a.e, j, n_j);
   const int i_end = min(a.M, iw + MB * 32);
-  Vec<T> res[2];   // this piece's and the next one's
+  Vec<T> res[2];
   res[0] = residual_vec<T>(a.e, iw + r0, j, iw + r0 < i_end ? n_j : 0);
   res[1] = residual_vec<T>(a.e, iw + r0 + STEP, j, iw + r0 + STEP < i_end ? n_j : 0);
   __syncthreads();
@@ -244,14 +242,21 @@ __device__ __forceinline__ void tile_end(const TileArgs& a, int split, int iw, i
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-    for (int q = 0; q < Q; ++q) {
-      const int r = r0 + q * STEP, i = iw + mm * 32 + r, ahead = i + 2 * STEP;
-      float z[V];
-      __builtin_memcpy(z, __builtin_assume_aligned(mine + r * STRIDE + c, 16), sizeof z);
-      const Vec<T> now = res[0];
-      res[0] = res[1];
-      res[1] = residual_vec<T>(a.e, ahead, j, ahead < i_end ? n_j : 0);
-      if (i < i_end && n_j > 0) finish_vec<T>(a.e, i, j, z, n_j, bias, now);
+    for (int q = 0; q < Q; q += 2) {   // two pieces at a time
+      float z[2][V];
+      Vec<T> now[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int r = r0 + (q + u) * STEP, ahead = iw + mm * 32 + r + 2 * STEP;
+        __builtin_memcpy(z[u], __builtin_assume_aligned(mine + r * STRIDE + c, 16), sizeof z[u]);
+        now[u] = res[u];
+        res[u] = residual_vec<T>(a.e, ahead, j, ahead < i_end ? n_j : 0);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int i = iw + mm * 32 + r0 + (q + u) * STEP;
+        if (i < i_end && n_j > 0) finish_vec<T>(a.e, i, j, z[u], n_j, bias, now[u]);
+      }
     }
   }
 }
@@ -308,15 +313,19 @@ struct Operand {
   int64_t ld;
   int left;          // i values in the tile
   int first;         // the stage's first value in its row
+  int lines;         // i values in the matrix
+  int back[ACROSS ? Q : 1];   // how far in front a piece that holds the last column is read
   Vec<T> reg[DEPTH][Q];   // stages under way
 
   __device__ __forceinline__ void init(const T* p, int64_t ld_, int i0, int n_i, int64_t k0) {
     ld = ld_;
     left = n_i - i0;
     first = ACROSS ? i0 : (int)k0;
+    lines = n_i;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int t = threadIdx.x + q * THREADS, line = t / PER_LINE, c = t % PER_LINE * V;
+      if (ACROSS) back[q] = c < left && left < c + V ? c + V - left : 0;
       // places outside the matrix read its nearest line or first piece instead: they only reach sums nobody stores
       if (ACROSS)
         ptr[q] = p + (k0 + line) * ld + i0 + (c < left ? c : 0);
@@ -325,16 +334,18 @@ struct Operand {
     }
   }
   // whether whole stages need no ends to be cut
-  __device__ __forceinline__ bool inside() const { return !ACROSS || left >= ROWS; }
+  __device__ __forceinline__ bool inside() const { return !ACROSS || lines >= V; }
   // the next stage, of which `have` (>= 1) r values exist, into reg[slot]; zeros behind them
   template <bool WHOLE>
   __device__ __forceinline__ void fetch(int slot, int have) {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int t = threadIdx.x + q * THREADS, line = t / PER_LINE, c = t % PER_LINE * V;
-      if (WHOLE)
+      if (WHOLE && (!ACROSS || left >= ROWS)) {
         reg[slot][q] = load_vec(ptr[q]);
-      else if (ACROSS)
+      } else if (WHOLE) {   // the last columns: read further in front, and shifted when they are stored
+        reg[slot][q] = load_vec(ptr[q] - back[q]);
+      } else if (ACROSS)
         reg[slot][q] = load_vec(ptr[q] - (line < have ? 0 : line * ld), line < have ? (c < left ? left - c : left) : 0, first + (c < left ? c : 0));
       else
         reg[slot][q] = load_vec(ptr[q] - (c < have ? 0 : c), have - c, first + c);
@@ -342,7 +353,7 @@ struct Operand {
     }
     if (!ACROSS) first += KT;
   }
-  __device__ __forceinline__ void store(char* lds, int slot) const {
+  __device__ __forceinline__ void store(char* lds, int slot, bool shifted) const {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int t = threadIdx.x + q * THREADS, line = t / PER_LINE, c = t % PER_LINE * V;
@@ -350,13 +361,20 @@ struct Operand {
       float rest[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) rest[i] = reg[slot][q].v[i];
+      if (ACROSS && shifted) {
+        const int b = back[q];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rest[i] = b & 2 ? (i < 2 ? rest[i + 2] : 0.0f) : rest[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rest[i] = b & 1 ? (i < 3 ? rest[i + 1] : 0.0f) : rest[i];
+      }
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         bf16_t term[4];
+        narrow<bf16_t, 4>(rest, term);
+        if (p + 1 < P) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          term[i] = (bf16_t)rest[i];
-          rest[i] -= (float)term[i];
+          for (int i = 0; i < 4; ++i) rest[i] -= (float)term[i];
         }
         __builtin_memcpy(__builtin_assume_aligned(dst + p * PLANE, 8), term, 8);
       }
@@ -462,6 +480,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile32(TileArgs a) {
     }
   };
   const int whole = A.inside() && B.inside() ? have / KT : 0;   // stages that need no ends to be cut
+  const bool a_edge = A_ACROSS && A.left < BM, b_edge = B_ACROSS && B.left < BN;
   auto fetch = [&](int slot, int stage) {
     if (stage < whole) {
       A.template fetch<true>(slot, KT);
@@ -472,14 +491,15 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile32(TileArgs a) {
     }
   };
   // stage s is multiplied from one buffer while s + 1 goes from its registers into the other and s + 1 + DEPTH is fetched
-  auto step = [&](int s, int u, auto whole) {
-    constexpr bool WHOLE = decltype(whole)::value;
+  auto step = [&](int s, int u, auto only_whole) {
+    constexpr bool WHOLE = decltype(only_whole)::value;
     __syncthreads();   // stage s is in LDS for everyone, stage s - 1 has been read by everyone
     const int buffer = DEPTH == 2 ? u : s & 1, slot = (u + 1) % DEPTH;
     multiply(buffer);
     if (WHOLE || s + 1 < stages) {
-      A.store(lds + (1 - buffer) * BUF, slot);
-      B.store(lds + (1 - buffer) * BUF + OpA::BYTES, slot);
+      const bool w = WHOLE || s + 1 < whole;
+      A.store(lds + (1 - buffer) * BUF, slot, w && a_edge);
+      B.store(lds + (1 - buffer) * BUF + OpA::BYTES, slot, w && b_edge);
     }
     if (WHOLE) {
       A.template fetch<true>(slot, KT);
@@ -497,8 +517,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile32(TileArgs a) {
     }
   };
   fetch(0, 0);
-  A.store(lds, 0);
-  B.store(lds + OpA::BYTES, 0);
+  A.store(lds, 0, whole > 0 && a_edge);
+  B.store(lds + OpA::BYTES, 0, whole > 0 && b_edge);
 #pragma unroll
   for (int d = 1; d <= DEPTH; ++d) fetch(d % DEPTH, d);
   int s = 0;
@@ -1011,8 +1031,7 @@ __global__ __launch_bounds__(256) void k_gate(GateArgs a) {
       }
       if (a.dz) {
         Vec<T> o;
-#pragma unroll
-        for (int i = 0; i < V; ++i) o.v[i] = (T)v[i];
+        narrow<T, V>(v, o.v);
         store_vec((T*)a.dz + r * a.ldz + col, o, n);
       }
 #pragma unroll

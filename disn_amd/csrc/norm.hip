@@ -113,7 +113,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm(NormArgs a) {
       if (c >= d) break;
       Vec<T> o;
 #pragma unroll
-      for (int i = 0; i < N; ++i) o.v[i] = (T)fmaf(x[p * N + i] * rstd, w[p * N + i], b[p * N + i]);
+      for (int i = 0; i < N; ++i) x[p * N + i] = fmaf(x[p * N + i] * rstd, w[p * N + i], b[p * N + i]);
+      narrow<T, N>(x + p * N, o.v);
       store_vec(y + c, o, EVEN ? N : d - c);
     }
   }
@@ -169,8 +170,9 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm_backward(NormA
         const int e = p * N + i;
         float v = rstd * (g[e] - s1 - h[e] * s2);
         if (a.residual) v += (float)rv[p].v[i];
-        o.v[i] = (T)v;
+        g[e] = v;
       }
+      narrow<T, N>(g + p * N, o.v);
       store_vec(dx + c, o, EVEN ? N : d - c);
     }
   }
