@@ -8,8 +8,8 @@
 //
 // Three kernels compute it, chosen by size (plan() below):
 //   k_tile16, k_tile32  large products: 128- or 256-wide tiles through LDS on the matrix cores
-//   k_small  products of a few tens of microseconds and less: no LDS tiles, the waves of a workgroup share the sum
-//   k_rows_* at most 16 rows times a large matrix: W streams past at memory speed
+//   k_small  products of some microseconds: no LDS tiles, the waves of a workgroup share the sum
+//   k_rows_* at most 4 rows times a large matrix: W streams past at memory speed
 #include "dense.h"
 
 #include <atomic>
@@ -884,8 +884,7 @@ __global__ __launch_bounds__(SMALL_WAVES * 64) void k_small_backward(SmallArgs d
 }
 
 // ---- k_rows: few rows times a large matrix ---------------------------------------------------------------------------
-// W is read once at memory speed, each value multiplied with MR rows of x (fp32 FMAs: 2 MR operations per value stay
-// below the vector rate up to 16 rows).  W by rows of r (across): a lane owns 16 bytes of columns, the workgroup's
+// W is read once at memory speed, each value multiplied with MR rows of x by fp32 FMAs.  W by rows of r (across): a lane owns 16 bytes of columns, the workgroup's
 // four waves share a range of r, ranges become partial sums for k_finish.
 struct RowsArgs {
   const void *x, *w;
@@ -1061,6 +1060,7 @@ struct Product {
 };
 struct Plan {
   Kind kind;
+  double us;                 // estimate
   int tile;                  // 128 or 256
   int splits;
   int64_t per;
@@ -1130,15 +1130,47 @@ Product rest_of(int type, Product q, int64_t cut) {
   return q;
 }
 
+// What k_small takes, in us; measured for 1 .. 256 rows and weights of 256^2 .. 4096^2.  Either one workgroup's chain of steps
+// along r bounds it (16-bit operands across r come in single values: 43 us at r = 4096, 6 at 1024), or the values that all
+// workgroups fetch: 3e6 a us in fp32 from L2, 1.75e6 from beyond it (weights of more than 32 MB), 2.4e6 in 16 bits.
+// Where an operand is gated, its slope is computed again in every workgroup that reads it: 0.4 of that rate (4099 rows
+// of 515 x 257, fp32 silu: 201 us for both gradients; 62 in tiles).
+double small_us(int type, const Product& q, bool gated = false) {
+  const int64_t mt = ceil_div(q.M, 16), nt = ceil_div(q.N, 16);
+  if (mt * nt > 1 << 20) return 1e30;
+  const bool f32 = type == DISN_F32;
+  const double K = (double)q.K, values = (double)mt * nt * 32 * K;
+  const double chain = f32 ? 0.0027 * K : q.a_across || q.b_across ? 2.5e-6 * K * K : 0.0023 * K;
+  const double rate = (f32 ? ((double)q.N * K > 8e6 ? 1.75e6 : 3e6) : 2.4e6) * (gated ? 0.4 : 1.0);
+  return 2.5 + (chain > values / rate ? chain : values / rate);
+}
+// The same of k_rows_*, up to four rows: W at 6.5 TB/s, and the sum of the parts as a launch more where W lies across r.
+// 4096 x 4096 in bf16 / fp32: one row 13.5 / 15.3 us across, 8.8 / 12.6 along r (k_small 43 / 22, 12 / 16; tiles 14 / 32),
+// four rows 15.4 / 16.9 and 14.2 / 19.3; eight rows 30 / 21 and 46 / 57, which the other kernels beat.
+double rows_us(int type, const Product& q) {
+  if (q.a_across || q.M > 4) return 1e30;
+  const int64_t size = (int64_t)dense_type_size(type);
+  const double read = (double)q.K * q.N * size / 6.5e6;
+  if (q.b_across) return 5.5 + read;
+  const double chain = 0.6 * q.K / (256 * 16 / size), us = read > chain ? read : chain;
+  return q.M > 1 ? 5.5 + 1.4 * us : 3.2 + us;
+}
+
 Plan plan(int type, const Product& q) {
   Plan p{};
   const bool a_across = q.a_across, b_across = q.b_across;
   const int64_t M = q.M, N = q.N, K = q.K;
   if (M == 0 || N == 0 || K == 0) return p;
   const int V = type == DISN_F32 ? 4 : 8, KT = type == DISN_F32 ? KT32 : KT16;
-  if (!a_across && M <= 16 && K * N >= (1 << 20)) {
-    p.kind = K_ROWS;
-    if (!b_across) return p;
+  const bool pack_a = type != DISN_F32 && !tile16_ready(q.A, q.lda), pack_b = type != DISN_F32 && !tile16_ready(q.B, q.ldb);
+  const TileChoice c = choose_tile(type == DISN_F32, M, N, K, !pack_a && !pack_b);
+  // (a copy of an operand takes 4 us and moves it twice)
+  const double tile = c.us + (pack_a ? 4 + 4e-6 * M * K / 4 : 0) + (pack_b ? 4 + 4e-6 * N * K / 4 : 0);
+  const double rows = rows_us(type, q), small = small_us(type, q);
+  p.us = rows < small ? rows : small;
+  if (p.us < tile) {
+    p.kind = rows < small ? K_ROWS : K_SMALL;
+    if (p.kind == K_SMALL || !b_across) return p;
     const int64_t groups = ceil_div(N, 64 * V);
     int64_t want = ceil_div(1024, groups);
     p.per = ceil_div(ceil_div(K, want), 32) * 32;
@@ -1147,13 +1179,7 @@ Plan plan(int type, const Product& q) {
     p.bytes = (size_t)p.splits * M * N * sizeof(float);
     return p;
   }
-  if ((double)M * N * K <= (1 << 27) && ceil_div(M, 16) * ceil_div(N, 16) <= (1 << 20)) {
-    p.kind = K_SMALL;
-    return p;
-  }
-  p.kind = K_TILE;
-  const bool pack_a = type != DISN_F32 && !tile16_ready(q.A, q.lda), pack_b = type != DISN_F32 && !tile16_ready(q.B, q.ldb);
-  const TileChoice c = choose_tile(type == DISN_F32, M, N, K, !pack_a && !pack_b);
+  p.kind = K_TILE, p.us = tile;
   p.tile = c.tile, p.splits = c.splits, p.cut = c.cut;
   p.per = ceil_div(ceil_div(K, p.splits), KT) * KT;
   p.splits = (int)ceil_div(K, p.per);
@@ -1275,8 +1301,7 @@ int run_product(DisnCtx* ctx, Product q, Plan p, char* ws, hipStream_t stream) {
   if (p.kind == K_ROWS) {
     RowsArgs r{q.A, q.B, q.lda, q.ldb, (int)q.M, (int)q.N, (int)q.K, (int)p.per, (int)ceil_div(q.N, 64 * Vec<T>::N), part, q.e};
     if (q.M == 1) launch_rows<T, 1>(r, q.b_across, p.splits, stream);
-    else if (q.M <= 4) launch_rows<T, 4>(r, q.b_across, p.splits, stream);
-    else launch_rows<T, 16>(r, q.b_across, p.splits, stream);
+    else launch_rows<T, 4>(r, q.b_across, p.splits, stream);
     DISN_HIP(ctx, hipGetLastError());
     return q.b_across ? launch_finish<T>(ctx, part, p.splits, q.M, q.N, q.e, stream) : DISN_OK;
   }
@@ -1355,7 +1380,10 @@ GradPlan plan_backward(const DisnLinearGrad* a) {
   else grad_products(a, a->dy, a->lddy, &dx, &dw);
   if (a->dx) g.dx = plan(a->type, dx);
   if (a->dw) g.dw = plan(a->type, dw);
-  g.small = a->dw && g.dw.kind == K_SMALL && (!a->dx || g.dx.kind == K_SMALL);
+  // one launch of k_small_backward, or dz and the bias's gradient first (two launches, 8 us and dz written and read)
+  const bool gated = a->act != DISN_ACT_NONE;
+  const double apart = g.dx.us + g.dw.us + 8 + 3e-6 * a->m * a->n * s / 5;
+  g.small = a->m && a->n && a->k && a->dw && (a->dx ? small_us(a->type, dx, gated) : 0) + small_us(a->type, dw, gated) <= apart;
   if (g.small) return g;
   const int V = (int)(16 / s);
   g.gate_lanes = 1;

@@ -555,9 +555,11 @@ def test_refusals_of_the_c_abi(ctx):
         assert linear(**bad) == (-1, -1), bad
         assert b"disn_linear" in lib.disn_last_error(h)
     assert lib.disn_linear(h, None, None, 0, None) == -1 and lib.disn_linear(None, None, None, 0, None) == -1
-    big = torch.ones(300, 2000, device=DEV)
-    a = _lib.DisnLinear(0, 0, 0, 0, 300, 300, 2000, big.data_ptr(), 2000, big.data_ptr(), 300, None, None, 0, p, 300, None, 0)
-    assert lib.disn_linear_workspace(h, ctypes.byref(a), ctypes.byref(n)) == 0 and n.value > 0
+    for k in (2000, 20000):   # a sum long enough to be split
+        big = torch.ones(300, k, device=DEV)
+        a = _lib.DisnLinear(0, 0, 0, 0, 300, 300, k, big.data_ptr(), k, big.data_ptr(), 300, None, None, 0, p, 300, None, 0)
+        assert lib.disn_linear_workspace(h, ctypes.byref(a), ctypes.byref(n)) == 0
+    assert n.value > 0
     ws = torch.empty(n.value + 16, dtype=torch.uint8, device=DEV)
     for ptr, size in ((None, 0), (ws.data_ptr(), n.value - 1), (ws.data_ptr() + 8, n.value)):
         assert lib.disn_linear(h, ctypes.byref(a), ptr, size, None) == -1
