@@ -1132,7 +1132,7 @@ Product rest_of(int type, Product q, int64_t cut) {
 
 // What k_small takes, in us; measured for 1 .. 256 rows and weights of 256^2 .. 4096^2.  Either one workgroup's chain of steps
 // along r bounds it (16-bit operands across r come in single values: 43 us at r = 4096, 6 at 1024), or the values that all
-// workgroups fetch: 3e6 a us in fp32 from L2, 1.75e6 from beyond it (weights of more than 32 MB), 2.4e6 in 16 bits.
+// workgroups fetch: 2.2e6 a us in fp32 from L2, 1.5e6 from beyond it (weights of more than 32 MB), 2e6 in 16 bits.
 // Where an operand is gated, its slope is computed again in every workgroup that reads it: 0.4 of that rate (4099 rows
 // of 515 x 257, fp32 silu: 201 us for both gradients; 62 in tiles).
 double small_us(int type, const Product& q, bool gated = false) {
@@ -1141,7 +1141,7 @@ double small_us(int type, const Product& q, bool gated = false) {
   const bool f32 = type == DISN_F32;
   const double K = (double)q.K, values = (double)mt * nt * 32 * K;
   const double chain = f32 ? 0.0027 * K : q.a_across || q.b_across ? 2.5e-6 * K * K : 0.0023 * K;
-  const double rate = (f32 ? ((double)q.N * K > 8e6 ? 1.75e6 : 3e6) : 2.4e6) * (gated ? 0.4 : 1.0);
+  const double rate = (f32 ? ((double)q.N * K > 8e6 ? 1.5e6 : 2.2e6) : 2e6) * (gated ? 0.4 : 1.0);
   return 2.5 + (chain > values / rate ? chain : values / rate);
 }
 // The same of k_rows_*, up to four rows: W at 6.5 TB/s, and the sum of the parts as a launch more where W lies across r.
