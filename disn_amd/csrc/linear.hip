@@ -633,6 +633,13 @@ struct Operand16 {
     }
     base += step;
   }
+  // piece p of the next stage, all of whose r values exist; after the last one, advance()
+  __device__ __forceinline__ void fetch_piece(char* dst, int p) const {
+    const unsigned m0 = (unsigned)(size_t)(lds_char*)dst + (threadIdx.x >> 6) * (PIECES * 1024) + p * 1024;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(m0)), "v"(off[p]), "s"(base)
+                 : "memory");
+  }
+  __device__ __forceinline__ void advance() { base += step; }
   // clears this lane's values behind the end of a landed stage
   __device__ __forceinline__ static void clear(char* dst, int have) {
 #pragma unroll
@@ -683,6 +690,7 @@ __global__ __launch_bounds__(WM * WN * 64, RING == 3 ? 3 : 2) void k_tile16(Tile
   constexpr int BUF = OpA::BYTES + OpB::BYTES, LOADS = OpA::PIECES + OpB::PIECES;
   static_assert(32 * tile_stride(NB) * 4 * WAVES <= RING * BUF, "the turned tiles fit into the ring");
   static_assert(RING == 3 || RING == 4, "waits");
+  static_assert(MB * NB >= MB + NB && MB * NB >= LOADS, "one fragment and one load a matrix instruction");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const TilePlace at = tile_place(a, BM, BN);
   const int64_t k0 = at.split * a.per;
@@ -737,7 +745,33 @@ __global__ __launch_bounds__(WM * WN * 64, RING == 3 ? 3 : 2) void k_tile16(Tile
     meet(0);
     fetch(RING - 1);
     read(0, 0);
-    for (int t = 0; t < whole; ++t) {
+    int t = 0;
+    // Where the stage to fetch exists and is whole: fragments and DMA are issued one after each matrix instruction, so that
+    // neither delays the next one (all of them behind the barrier left the matrix cores idle for a fifth of a stage).
+    for (; t + RING < whole; ++t) {
+      const char *cur = slot(t), *next = slot(t + 1);
+      char* dst = slot(t);
+#pragma unroll
+      for (int i = 0; i < MB * NB; ++i) {
+        acc[i / NB][i % NB] = mfma<T>(fa[0][i / NB], fb[0][i % NB], acc[i / NB][i % NB]);
+        if (i < NB) fb[1][i] = OpB::fragment(cur + OpA::BYTES, ob, i, 1);
+        else if (i < NB + MB) fa[1][i - NB] = OpA::fragment(cur, oa, i - NB, 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * LOADS) : "memory");
+#pragma unroll
+      for (int i = 0; i < MB * NB; ++i) {
+        acc[i / NB][i % NB] = mfma<T>(fa[1][i / NB], fb[1][i % NB], acc[i / NB][i % NB]);
+        if (i < NB) fb[0][i] = OpB::fragment(next + OpA::BYTES, ob, i, 0);
+        else if (i < NB + MB) fa[0][i - NB] = OpA::fragment(next, oa, i - NB, 0);
+        if (i < OpA::PIECES) A.fetch_piece(dst, i);
+        else if (i < LOADS) B.fetch_piece(dst + OpA::BYTES, i - OpA::PIECES);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      A.advance();
+      B.advance();
+    }
+    for (; t < whole; ++t) {
       read(t, 1);
       multiply(0);
       if (t + 1 < whole) {
