@@ -1144,13 +1144,13 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // How a large product is cut into workgroups: 128- or 256-wide tiles, r split into `splits` parts or not.  A CU holds one
 // workgroup with 256-wide tiles (its LDS), two with 128-wide ones, or three of those with a ring of three stages.  A round of
-// them costs a fixed time and a time per r value; measured (us, ns per r), 2048 .. 65536 x 512 .. 4096, r = 128 .. 2048:
-//              256-wide     128-wide: one a CU    two         three
-//   16 bits    12, 26                 7, 10.4     9, 17       7.5, 24
-//   fp32       22, 150                13, 73      13, 90
-// Split sums are written and read once more in fp32, at 5 TB/s, by one more launch (4 us).  The estimates are within 15 % of
-// what was measured: gradient of a 1536 x 512 weight over 65536 bf16 rows 256-wide / 21 parts 123 (121 measured), 128-wide / 10
-// parts 137 (135); 65536 x 512 outputs with r = 128 256-wide 31 (32), 128-wide 29 (28), r = 1536 103 (113), 118 (120).
+// them costs a fixed time and a time per r value; measured (us, ns per r), 2048 .. 8192 x 1024 .. 4096, r = 512 and 2048:
+//              256-wide: half the chip, all of it    128-wide: one a CU    two         three
+//   16 bits    9.5, 17                 9.5, 25                 5.5, 7.5     7, 16.5     7.7, 25.5
+//   fp32       14, 105                 14, 145                 9.2, 50      9, 85
+// Split sums are written and read once more in fp32, at 10 TB/s while they fit the last cache, by one more launch (4 us).
+// Measured (estimated): gradient of a 1536 x 512 weight over 65536 bf16 rows 256-wide / 21 parts 103 (105), 128-wide / 10 parts
+// 127 (125); 4096 x 4096, r = 2048 256-wide 61 (61), 128-wide 86 (81); 2048 x 2048, r = 2048, 256-wide / 4 parts 39 (40).
 // A last round that is at most half full is not started (operands that are copied first aside): the rows before it are one
 // launch, the others another (100000 x 512 fp32 outputs are 782 tiles, three rounds and 14 tiles).
 struct TileChoice {
@@ -1159,10 +1159,14 @@ struct TileChoice {
   double us;
 };
 double tile_rounds_us(bool f32, int tile, int64_t blocks, double r) {
-  if (tile == 256) return (double)ceil_div(blocks, 256) * (f32 ? 22 + 0.15 * r : 12 + 0.026 * r);
-  const double one = f32 ? 13 + 0.073 * r : 7 + 0.0104 * r, two = f32 ? 13 + 0.09 * r : 9 + 0.017 * r;
+  if (tile == 256) {
+    const double fill = (double)(blocks % 256) / 256, rounds = (double)(blocks / 256);
+    return f32 ? rounds * (14 + 0.145 * r) + (fill > 0 ? 14 + (0.065 + 0.08 * fill) * r : 0)
+               : rounds * (9.5 + 0.025 * r) + (fill > 0 ? 9.5 + (0.009 + 0.016 * fill) * r : 0);
+  }
+  const double one = f32 ? 9.2 + 0.05 * r : 5.5 + 0.0075 * r, two = f32 ? 9 + 0.085 * r : 7 + 0.0165 * r;
   const int64_t full = f32 ? 512 : 768, last = blocks > 512 ? blocks % full : blocks;
-  const double three = 7.5 + 0.024 * r, whole = blocks > 512 ? (double)(blocks / full) * (f32 ? two : three) : 0;
+  const double three = 7.7 + 0.0255 * r, whole = blocks > 512 ? (double)(blocks / full) * (f32 ? two : three) : 0;
   return whole + (last == 0 ? 0 : last <= 256 ? one : last <= 512 ? two : three);
 }
 TileChoice choose_tile(bool f32, int64_t M, int64_t N, int64_t K, bool may_cut) {
@@ -1173,13 +1177,15 @@ TileChoice choose_tile(bool f32, int64_t M, int64_t N, int64_t K, bool may_cut) 
       const int64_t blocks = tiles * s;
       if (s > 1 && (K / s < 128 || blocks > 768)) break;
       double us = tile_rounds_us(f32, tile, blocks, (double)ceil_div(K, s));
-      if (s > 1) us += 4 + 8e-6 * s * M * N / 5;
+      const double moved = 8e-6 * s * M * N;   // MB
+      if (s > 1) us += 4 + moved / (moved < 256 ? 10 : 7);
       if (us < best.us) best = {tile, s, 0, us};
     }
   }
   const int64_t nt = ceil_div(N, 256), tiles = ceil_div(M, 256) * nt, over = tiles % 256;
   if (may_cut && tiles > 256 && over > 0 && over <= 128) {
     const int64_t cut = (tiles - over) / nt * 256;   // whole rows of tiles
+    if (cut == 0) return best;
     const double us = tile_rounds_us(f32, 256, cut / 256 * nt, (double)K) + 4 + choose_tile(f32, M - cut, N, K, false).us;
     if (us < best.us) best = {256, 1, cut, us};
   }

@@ -26,7 +26,8 @@ ACTS = ("none", "relu", "gelu", "silu")
 # short sums; tiles of 128 and 256, split and whole, with edges in every direction
 SIZES = [(0, 5, 4), (5, 0, 4), (3, 5, 0), (1, 1, 1), (1, 2, 7), (7, 3, 64), (17, 129, 33), (33, 515, 257), (24, 1024, 512), (16, 127, 128),
          (1, 4096, 260), (2, 1031, 1025), (5, 2049, 515), (16, 1024, 1024), (17, 1024, 1024), (1, 70000, 16), (3, 16, 70000),
-         (1000, 300, 777), (130, 1032, 1025), (4099, 515, 257), (65, 20000, 130), (33000, 65, 520), (20000, 67, 1000)]
+         (1000, 300, 777), (130, 1032, 1025), (4099, 515, 257), (65, 20000, 130), (33000, 65, 520), (20000, 67, 1000),
+         (3, 4096, 2100), (4, 2000, 3000), (3000, 900, 1100), (9000, 1100, 2000), (66000, 700, 520)]
 
 
 def ints(gen, kind, *shape, top=3):
@@ -114,7 +115,7 @@ def test_linear_backward_parts(ctx, m, k, n, want):
 
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("kind", list(KINDS))
-@pytest.mark.parametrize("m,k,n", [(1, 3, 5), (24, 1024, 512), (4, 1500, 800), (700, 1100, 333), (33000, 40, 520)])
+@pytest.mark.parametrize("m,k,n", [(1, 3, 5), (24, 1024, 512), (4, 1500, 800), (700, 1100, 333), (33000, 40, 520), (3000, 900, 1100)])
 def test_linear_values(ctx, m, k, n, kind, act):
     g = gen(m, k, n, kind, act)
     x, w, b, r = (torch.randn(*s, generator=g, device=DEV).to(KINDS[kind]) for s in ((m, k), (k, n), (n,), (m, n)))
@@ -132,7 +133,7 @@ def test_linear_values(ctx, m, k, n, kind, act):
 
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("kind", list(KINDS))
-@pytest.mark.parametrize("m,k,n", [(1, 3, 5), (32, 1024, 512), (900, 300, 520), (5000, 130, 260), (9, 1100, 1000)])
+@pytest.mark.parametrize("m,k,n", [(1, 3, 5), (32, 1024, 512), (900, 300, 520), (5000, 130, 260), (9, 1100, 1000), (3000, 900, 1100)])
 def test_linear_backward_values(ctx, m, k, n, kind, act):
     g = gen(m, k, n, kind, act, 2)
     x, w, dy, pre = (torch.randn(*s, generator=g, device=DEV).to(KINDS[kind]) for s in ((m, k), (k, n), (m, n), (m, n)))
@@ -173,7 +174,7 @@ def test_linear_gradient_against_differences(ctx, m, k, n, act):
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
-@pytest.mark.parametrize("m,k,n", [(5, 40, 30), (3, 1100, 1000), (300, 700, 800), (33000, 40, 520)])
+@pytest.mark.parametrize("m,k,n", [(5, 40, 30), (3, 1100, 1000), (300, 700, 800), (33000, 40, 520), (3, 4096, 2100), (3000, 900, 1100), (9000, 1100, 2000)])
 def test_linear_rows_anywhere(ctx, m, k, n, kind):
     """slices of wider buffers at odd addresses, expanded and transposed inputs, a column range as the output"""
     g = gen(m, k, n, kind, 4)
@@ -223,7 +224,7 @@ def test_linear_leading_dimensions(ctx):
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
-@pytest.mark.parametrize("m,k,n", [(20, 40, 30), (4, 1100, 1000), (300, 700, 800)])
+@pytest.mark.parametrize("m,k,n", [(20, 40, 30), (4, 1100, 1000), (300, 700, 800), (4, 4096, 2100), (3000, 900, 1100), (9000, 1100, 2000)])
 def test_linear_infinities_and_nan(ctx, m, k, n, kind):
     """they reach exactly the sums that hold them, as in a chain of multiply-adds"""
     g = gen(m, k, n, kind, 6)
@@ -242,7 +243,7 @@ def test_linear_infinities_and_nan(ctx, m, k, n, kind):
     assert torch.equal(relu[1].isinf(), w[7] > 0) and (relu[1][w[7] < 0] == 0).all()
 
 
-@pytest.mark.parametrize("m,k,n", [(20, 40, 30), (4, 1100, 1000), (300, 700, 800)])
+@pytest.mark.parametrize("m,k,n", [(20, 40, 30), (4, 1100, 1000), (300, 700, 800), (3, 4096, 2100), (3000, 900, 1100), (9000, 1100, 2000)])
 def test_linear_float32_range(ctx, m, k, n):
     """the whole range of float32: values next to the largest, sums that overflow, products that are subnormal"""
     g = gen(m, k, n, 7)
