@@ -300,9 +300,9 @@ __device__ __forceinline__ void tile_end(const TileArgs& a, int split, int iw, i
 struct TilePlace {
   int i0, j0, split;
 };
-__device__ __forceinline__ TilePlace tile_place(const TileArgs& a, int BM, int BN) {
-  const int total = a.mt * a.nt * a.splits, run = total >> 3, rest = total & 7, xcd = blockIdx.x & 7;
-  int id = (blockIdx.x >> 3) + xcd * run + (xcd < rest ? xcd : rest);
+__device__ __forceinline__ TilePlace tile_place(const TileArgs& a, int block, int BM, int BN) {
+  const int total = a.mt * a.nt * a.splits, run = total >> 3, rest = total & 7, xcd = block & 7;
+  int id = (block >> 3) + xcd * run + (xcd < rest ? xcd : rest);
   const int tn = id % a.nt;
   id /= a.nt;
   return {id % a.mt * BM, tn * BN, id / a.mt};
@@ -462,13 +462,12 @@ __device__ __forceinline__ void fma_tile(const TileArgs& a, bool a_across, bool 
 }
 
 template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int DEPTH>
-__global__ __launch_bounds__(WM * WN * 64, 2) void k_tile32(TileArgs a) {
+__device__ __forceinline__ void tile32(const TileArgs& a, int block, char* lds) {
   constexpr int THREADS = WM * WN * 64, MB = BM / WM / 32, NB = BN / WN / 32, KT = KT32, P = PLANES;
   typedef Operand<T, A_ACROSS, BM, THREADS, DEPTH> OpA;
   typedef Operand<T, B_ACROSS, BN, THREADS, DEPTH> OpB;
   constexpr int BUF = OpA::BYTES + OpB::BYTES;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  const TilePlace at = tile_place(a, BM, BN);
+  const TilePlace at = tile_place(a, block, BM, BN);
   const int i0 = at.i0, j0 = at.j0, split = at.split;
   const int64_t k0 = split * a.per;
   const int have = (int)(a.K - k0 < a.per ? a.K - k0 : a.per), stages = (have + KT - 1) / KT;
@@ -581,6 +580,12 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile32(TileArgs a) {
   tile_end<T, MB, NB, WM * WN>(a, split, i0 + wi, j0 + wj, acc, (float*)lds);
 }
 
+template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int DEPTH>
+__global__ __launch_bounds__(WM * WN * 64, 2) void k_tile32(TileArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  tile32<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN, DEPTH>(a, blockIdx.x, lds);
+}
+
 // ---- k_tile16 ------------------------------------------------------------------------------------------------------
 // bf16 and fp16.  A ring of LDS stages of 32 r is filled by DMA (global_load_lds_dwordx4: no registers, no LDS store
 // instructions), so all but one of its stages are on their way while one is multiplied.  Two steps of 16 r a stage, and
@@ -683,7 +688,7 @@ struct Operand16 {
 };
 
 template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int RING>
-__global__ __launch_bounds__(WM * WN * 64, RING == 3 ? 3 : 2) void k_tile16(TileArgs a) {
+__device__ __forceinline__ void tile16(const TileArgs& a, int block, char* lds) {
   constexpr int WAVES = WM * WN, MB = BM / WM / 32, NB = BN / WN / 32;
   typedef Operand16<T, A_ACROSS, BM, WAVES, MB> OpA;
   typedef Operand16<T, B_ACROSS, BN, WAVES, NB> OpB;
@@ -691,8 +696,7 @@ __global__ __launch_bounds__(WM * WN * 64, RING == 3 ? 3 : 2) void k_tile16(Tile
   static_assert(32 * tile_stride(NB) * 4 * WAVES <= RING * BUF, "the turned tiles fit into the ring");
   static_assert(RING == 3 || RING == 4, "waits");
   static_assert(MB * NB >= MB + NB && MB * NB >= LOADS, "one fragment and one load a matrix instruction");
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  const TilePlace at = tile_place(a, BM, BN);
+  const TilePlace at = tile_place(a, block, BM, BN);
   const int64_t k0 = at.split * a.per;
   const int have = (int)(a.K - k0 < a.per ? a.K - k0 : a.per), whole = have / KT16, rest = have % KT16, stages = whole + (rest ? 1 : 0);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave / WN * (MB * 32), wj = wave % WN * (NB * 32);
@@ -793,6 +797,27 @@ __global__ __launch_bounds__(WM * WN * 64, RING == 3 ? 3 : 2) void k_tile16(Tile
     multiply(1);
   }
   tile_end<T, MB, NB, WAVES>(a, at.split, at.i0 + wi, at.j0 + wj, acc, (float*)lds);
+}
+
+template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int RING>
+__global__ __launch_bounds__(WM * WN * 64, RING == 3 ? 3 : 2) void k_tile16(TileArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  tile16<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN, RING>(a, blockIdx.x, lds);
+}
+
+// Both gradients of a layer in one launch where neither fills the chip: the first `split` workgroups compute dx, the others dW
+// (4099 rows of 515 x 257 in fp32, 165 and 255 workgroups: 50 us one after the other).
+template <typename T, bool W_NK>
+__global__ __launch_bounds__(256, 2) void k_tile_pair(TileArgs dx, TileArgs dw, int split) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int block = blockIdx.x;
+  if constexpr (sizeof(T) == 4) {
+    if (block < split) tile32<T, false, W_NK, 128, 128, 2, 2, 2>(dx, block, lds);
+    else tile32<T, true, true, 128, 128, 2, 2, 2>(dw, block - split, lds);
+  } else {
+    if (block < split) tile16<T, false, W_NK, 128, 128, 2, 2, 4>(dx, block, lds);
+    else tile16<T, true, true, 128, 128, 2, 2, 4>(dw, block - split, lds);
+  }
 }
 
 // a copy of a 16-bit matrix on 16-byte boundaries
@@ -1084,9 +1109,32 @@ __global__ __launch_bounds__(256) void k_gate(GateArgs a) {
   float s[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) s[i] = 0.0f;
+  int64_t r = rb * a.rows_per + line;
+  if ((group + 1) * L * V <= a.N) {   // whole pieces: four rows under way
+    for (; r + 3 * lines < r1; r += 4 * lines) {
+      Vec<T> g[4], z[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        g[u] = load_vec((const T*)a.dy + (r + u * lines) * a.lddy + col);
+        if (a.act != DISN_ACT_NONE) z[u] = load_vec((const T*)a.pre + (r + u * lines) * a.ldp + col);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float v[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = (float)g[u].v[i] * (a.act != DISN_ACT_NONE ? slope((float)z[u].v[i], a.act) : 1.0f);
+        if (a.dz) {
+          Vec<T> o;
+          narrow<T, V>(v, o.v);
+          store_vec((T*)a.dz + (r + u * lines) * a.ldz + col, o, V);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] += v[i];
+      }
+    }
+  }
   if (n > 0) {
-#pragma unroll 4
-    for (int64_t r = rb * a.rows_per + line; r < r1; r += lines) {
+    for (; r < r1; r += lines) {
       const Vec<T> g = load_vec((const T*)a.dy + r * a.lddy + col, n, col);
       float v[V];
 #pragma unroll
@@ -1282,35 +1330,52 @@ int launch_finish(DisnCtx* ctx, const float* part, int nparts, int64_t M, int64_
   return DISN_OK;
 }
 
-template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int RING>
-int launch_tile(DisnCtx* ctx, const TileArgs& a, hipStream_t stream) {
-  constexpr int THREADS = WM * WN * 64;
-  const void* kernel;
-  int bytes;
-  if constexpr (sizeof(T) == 4) {
-    constexpr int DEPTH = BM == 128 ? 2 : 1;   // a stage of a 128-wide tile is over before the next has come
-    kernel = (const void*)k_tile32<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN, DEPTH>;
-    bytes = 2 * (Operand<T, A_ACROSS, BM, THREADS, DEPTH>::BYTES + Operand<T, B_ACROSS, BN, THREADS, DEPTH>::BYTES);
-  } else {
-    kernel = (const void*)k_tile16<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN, RING>;
-    bytes = RING * (BM + BN) * KT16 * 2;
-  }
-  static std::atomic<uint64_t> ready{0};   // devices that allow this kernel its LDS
+// LDS of a tile's workgroup
+template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int THREADS, int RING>
+constexpr int tile_lds() {
+  if constexpr (sizeof(T) == 4)
+    return 2 * (Operand<T, A_ACROSS, BM, THREADS, 1>::BYTES + Operand<T, B_ACROSS, BN, THREADS, 1>::BYTES);
+  else
+    return RING * (BM + BN) * KT16 * 2;
+}
+// launches a kernel that needs more LDS than a kernel may have unasked; ready: devices that have been asked
+int launch_lds(DisnCtx* ctx, std::atomic<uint64_t>& ready, const void* kernel, int64_t blocks, int threads, void** args, int bytes,
+               hipStream_t stream) {
   const uint64_t bit = 1ull << (ctx->device & 63);
   if (!(ready.load() & bit)) {
     DISN_HIP(ctx, hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     ready.fetch_or(bit);
   }
-  TileArgs copy = a;
-  void* args[] = {&copy};
-  DISN_HIP(ctx, hipLaunchKernel(kernel, dim3((unsigned)((int64_t)a.mt * a.nt * a.splits)), dim3(THREADS), args, bytes, stream));
+  DISN_HIP(ctx, hipLaunchKernel(kernel, dim3((unsigned)blocks), dim3(threads), args, bytes, stream));
   return DISN_OK;
+}
+int64_t tile_blocks(const TileArgs& a) { return (int64_t)a.mt * a.nt * a.splits; }
+
+template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int RING>
+int launch_tile(DisnCtx* ctx, TileArgs a, hipStream_t stream) {
+  constexpr int THREADS = WM * WN * 64;
+  const void* kernel;
+  if constexpr (sizeof(T) == 4)   // (a stage of a 128-wide tile is over before the next has come: two under way)
+    kernel = (const void*)k_tile32<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN, BM == 128 ? 2 : 1>;
+  else
+    kernel = (const void*)k_tile16<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN, RING>;
+  static std::atomic<uint64_t> ready{0};
+  void* args[] = {&a};
+  return launch_lds(ctx, ready, kernel, tile_blocks(a), THREADS, args, tile_lds<T, A_ACROSS, B_ACROSS, BM, BN, THREADS, RING>(), stream);
+}
+template <typename T, bool W_NK>
+int launch_pair(DisnCtx* ctx, TileArgs dx, TileArgs dw, hipStream_t stream) {
+  constexpr int x = tile_lds<T, false, W_NK, 128, 128, 256, 4>(), w = tile_lds<T, true, true, 128, 128, 256, 4>();
+  static std::atomic<uint64_t> ready{0};
+  int split = (int)tile_blocks(dx);
+  void* args[] = {&dx, &dw, &split};
+  return launch_lds(ctx, ready, (const void*)k_tile_pair<T, W_NK>, split + tile_blocks(dw), 256, args, x > w ? x : w, stream);
 }
 template <typename T, bool A_ACROSS, bool B_ACROSS>
 int launch_tile(DisnCtx* ctx, int tile, const TileArgs& a, hipStream_t stream) {
   if (tile == 256) return launch_tile<T, A_ACROSS, B_ACROSS, 256, 256, 2, 4, 4>(ctx, a, stream);
   if constexpr (sizeof(T) == 2)   // 48 KB of LDS: three a CU
-    if ((int64_t)a.mt * a.nt * a.splits > 512) return launch_tile<T, A_ACROSS, B_ACROSS, 128, 128, 2, 2, 3>(ctx, a, stream);
+    if (tile_blocks(a) > 512) return launch_tile<T, A_ACROSS, B_ACROSS, 128, 128, 2, 2, 3>(ctx, a, stream);
   return launch_tile<T, A_ACROSS, B_ACROSS, 128, 128, 2, 2, 4>(ctx, a, stream);
 }
 // a copy of rows x cols values at dst, 16-byte boundaries; *p, *ld become it
@@ -1342,6 +1407,18 @@ SmallArgs small_args(const Product& q, const Plan&) {
 }
 int64_t small_blocks(const SmallArgs& s) { return (int64_t)s.mt * ceil_div(s.nt, SMALL_WAVES / s.ks); }
 
+// a product in tiles: copies what has to be copied and fills in the kernel's arguments
+template <typename T>
+int prepare_tile(DisnCtx* ctx, Product q, const Plan& p, char* ws, TileArgs* t, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    if (p.pack_a) DISN_TRY(launch_pack<T>(ctx, &q.A, &q.lda, q.a_across ? q.K : q.M, q.a_across ? q.M : q.K, ws, stream));
+    if (p.pack_b) DISN_TRY(launch_pack<T>(ctx, &q.B, &q.ldb, q.b_across ? q.K : q.N, q.b_across ? q.N : q.K, ws + p.pack_a, stream));
+  }
+  *t = {q.A, q.B, q.lda, q.ldb, (int)q.M, (int)q.N, q.K, p.per, (int)ceil_div(q.M, p.tile), (int)ceil_div(q.N, p.tile), p.splits,
+        (float*)(ws + p.pack_a + p.pack_b), q.e};
+  return DISN_OK;
+}
+
 // one product by its plan; ws: plan.bytes of workspace
 template <typename T>
 int run_product(DisnCtx* ctx, Product q, Plan p, char* ws, hipStream_t stream) {
@@ -1351,11 +1428,7 @@ int run_product(DisnCtx* ctx, Product q, Plan p, char* ws, hipStream_t stream) {
     q.M = p.cut;
     p.cut = 0;
   }
-  float* part = (float*)(ws + p.pack_a + p.pack_b);
-  if constexpr (sizeof(T) == 2) {
-    if (p.pack_a) DISN_TRY(launch_pack<T>(ctx, &q.A, &q.lda, q.a_across ? q.K : q.M, q.a_across ? q.M : q.K, ws, stream));
-    if (p.pack_b) DISN_TRY(launch_pack<T>(ctx, &q.B, &q.ldb, q.b_across ? q.K : q.N, q.b_across ? q.N : q.K, ws + p.pack_a, stream));
-  }
+  float* part = (float*)ws;
   if (q.M == 0 || q.N == 0) return DISN_OK;
   if (p.kind == K_EMPTY) return launch_finish<T>(ctx, nullptr, 0, q.M, q.N, q.e, stream);
   if (p.kind == K_SMALL) {
@@ -1379,12 +1452,12 @@ int run_product(DisnCtx* ctx, Product q, Plan p, char* ws, hipStream_t stream) {
     DISN_HIP(ctx, hipGetLastError());
     return q.b_across ? launch_finish<T>(ctx, part, p.splits, q.M, q.N, q.e, stream) : DISN_OK;
   }
-  TileArgs t{q.A, q.B, q.lda, q.ldb, (int)q.M, (int)q.N, q.K, p.per, (int)ceil_div(q.M, p.tile), (int)ceil_div(q.N, p.tile), p.splits,
-             part, q.e};
+  TileArgs t;
+  DISN_TRY(prepare_tile<T>(ctx, q, p, ws, &t, stream));
   if (q.a_across) DISN_TRY((launch_tile<T, true, true>(ctx, p.tile, t, stream)));
   else if (q.b_across) DISN_TRY((launch_tile<T, false, true>(ctx, p.tile, t, stream)));
   else DISN_TRY((launch_tile<T, false, false>(ctx, p.tile, t, stream)));
-  return p.splits > 1 ? launch_finish<T>(ctx, part, p.splits, q.M, q.N, q.e, stream) : DISN_OK;
+  return p.splits > 1 ? launch_finish<T>(ctx, t.part, p.splits, q.M, q.N, q.e, stream) : DISN_OK;
 }
 
 // ---- host: arguments -----------------------------------------------------------------------------------------------------
@@ -1430,9 +1503,10 @@ Product forward_product(const DisnLinear* a) {
           {a->bias, a->residual, a->pre, a->y, a->ldr, a->ldp, a->ldy, a->act}};
 }
 
-// The backward pass of one call: small ones are one launch; others write dz once (act != none), then two products.
+// The backward pass of one call: small ones are one launch; others write dz once (act != none), then two products, at once
+// where they fit the chip together.
 struct GradPlan {
-  bool small;
+  bool small, pair;
   Plan dx, dw;
   int64_t ldz, gate_blocks, gate_rows;
   int gate_lanes, gate_groups;
@@ -1476,7 +1550,12 @@ GradPlan plan_backward(const DisnLinearGrad* a) {
   g.off_sums = at;
   if (a->db) at += align256((size_t)g.gate_blocks * a->n * sizeof(float));
   g.off_part = at;
-  at += g.dx.bytes > g.dw.bytes ? g.dx.bytes : g.dw.bytes;
+  // both products at once where they are 128-wide tiles that fit the chip together, two a CU
+  auto blocks128 = [](const Plan& p, const Product& q) {
+    return p.kind == K_TILE && p.tile == 128 && !p.cut ? ceil_div(q.M, 128) * ceil_div(q.N, 128) * p.splits : 1 << 30;
+  };
+  g.pair = a->dx && a->dw && blocks128(g.dx, dx) + blocks128(g.dw, dw) <= 512;
+  at += g.pair ? align256(g.dx.bytes) + g.dw.bytes : g.dx.bytes > g.dw.bytes ? g.dx.bytes : g.dw.bytes;
   g.bytes = at;
   return g;
 }
@@ -1503,6 +1582,16 @@ int run_backward(DisnCtx* ctx, const DisnLinearGrad* a, const GradPlan& g, char*
   }
   Product dx, dw;
   grad_products(a, dz, ldz, &dx, &dw);
+  if (g.pair) {
+    TileArgs tx, tw;
+    DISN_TRY(prepare_tile<T>(ctx, dx, g.dx, ws + g.off_part, &tx, stream));
+    DISN_TRY(prepare_tile<T>(ctx, dw, g.dw, ws + g.off_part + align256(g.dx.bytes), &tw, stream));
+    if (a->w_nk) DISN_TRY((launch_pair<T, true>(ctx, tx, tw, stream)));
+    else DISN_TRY((launch_pair<T, false>(ctx, tx, tw, stream)));
+    if (g.dx.splits > 1) DISN_TRY(launch_finish<T>(ctx, tx.part, g.dx.splits, dx.M, dx.N, dx.e, stream));
+    if (g.dw.splits > 1) DISN_TRY(launch_finish<T>(ctx, tw.part, g.dw.splits, dw.M, dw.N, dw.e, stream));
+    return DISN_OK;
+  }
   if (!g.small) {
     if (a->dx) DISN_TRY(run_product<T>(ctx, dx, g.dx, ws + g.off_part, stream));
     if (a->dw) DISN_TRY(run_product<T>(ctx, dw, g.dw, ws + g.off_part, stream));
