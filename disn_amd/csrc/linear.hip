@@ -1221,13 +1221,14 @@ TileChoice choose_tile(bool f32, int64_t M, int64_t N, int64_t K, bool may_cut) 
   TileChoice best{0, 0, 0, 1e30};
   for (int tile = 256; tile >= 128; tile /= 2) {
     const int64_t tiles = ceil_div(M, tile) * ceil_div(N, tile);
-    for (int s = 1; s <= 64; ++s) {
-      const int64_t blocks = tiles * s;
-      if (s > 1 && (K / s < 128 || blocks > 768)) break;
-      double us = tile_rounds_us(f32, tile, blocks, (double)ceil_div(K, s));
+    // not split, a few parts, as many as fill the chip in one, two or three workgroups a CU, or as many as the sum allows
+    const int64_t parts[] = {1, 2, 3, 4, 128 / tiles, 256 / tiles, 512 / tiles, 768 / tiles, K / 256, K / 128};
+    for (const int64_t s : parts) {
+      if (s < 1 || (s > 1 && (K / s < 128 || tiles * s > 768))) continue;
+      double us = tile_rounds_us(f32, tile, tiles * s, (double)ceil_div(K, s));
       const double moved = 8e-6 * s * M * N;   // MB
       if (s > 1) us += 4 + moved / (moved < 256 ? 10 : 7);
-      if (us < best.us) best = {tile, s, 0, us};
+      if (us < best.us) best = {tile, (int)s, 0, us};
     }
   }
   const int64_t nt = ceil_div(N, 256), tiles = ceil_div(M, 256) * nt, over = tiles % 256;
@@ -1528,9 +1529,15 @@ GradPlan plan_backward(const DisnLinearGrad* a) {
   else grad_products(a, a->dy, a->lddy, &dx, &dw);
   if (a->dx) g.dx = plan(a->type, dx);
   if (a->dw) g.dw = plan(a->type, dw);
+  // both products at once where they are 128-wide tiles that fit the chip together, two a CU
+  auto blocks128 = [](const Plan& p, const Product& q) {
+    return p.kind == K_TILE && p.tile == 128 && !p.cut ? ceil_div(q.M, 128) * ceil_div(q.N, 128) * p.splits : 1 << 30;
+  };
+  g.pair = a->dx && a->dw && blocks128(g.dx, dx) + blocks128(g.dw, dw) <= 512;
   // one launch of k_small_backward, or dz and the bias's gradient first (two launches, 8 us and dz written and read)
   const bool gated = a->act != DISN_ACT_NONE;
-  const double apart = g.dx.us + g.dw.us + 8 + 3e-6 * a->m * a->n * s / 5;
+  const double products = !g.pair ? g.dx.us + g.dw.us : g.dx.us > g.dw.us ? g.dx.us + 3 : g.dw.us + 3;
+  const double apart = products + 8 + 3e-6 * a->m * a->n * s / 5;
   g.small = a->m && a->n && a->k && a->dw && (a->dx ? small_us(a->type, dx, gated) : 0) + small_us(a->type, dw, gated) <= apart;
   if (g.small) return g;
   const int V = (int)(16 / s);
@@ -1550,11 +1557,6 @@ GradPlan plan_backward(const DisnLinearGrad* a) {
   g.off_sums = at;
   if (a->db) at += align256((size_t)g.gate_blocks * a->n * sizeof(float));
   g.off_part = at;
-  // both products at once where they are 128-wide tiles that fit the chip together, two a CU
-  auto blocks128 = [](const Plan& p, const Product& q) {
-    return p.kind == K_TILE && p.tile == 128 && !p.cut ? ceil_div(q.M, 128) * ceil_div(q.N, 128) * p.splits : 1 << 30;
-  };
-  g.pair = a->dx && a->dw && blocks128(g.dx, dx) + blocks128(g.dw, dw) <= 512;
   at += g.pair ? align256(g.dx.bytes) + g.dw.bytes : g.dx.bytes > g.dw.bytes ? g.dx.bytes : g.dw.bytes;
   g.bytes = at;
   return g;
