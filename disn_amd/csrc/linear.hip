@@ -638,7 +638,8 @@ struct Operand16 {
     }
     base += step;
   }
-  // piece p of the next stage, all of whose r values exist; after the last one, advance()
+  // piece p of the next stage, all of whose r values exist; after the last one, advance().  M0 holds a DMA's LDS address;
+  // hipcc has no use of its own for it here (LDS instructions of gfx9 do not read it).
   __device__ __forceinline__ void fetch_piece(char* dst, int p) const {
     const unsigned m0 = (unsigned)(size_t)(lds_char*)dst + (threadIdx.x >> 6) * (PIECES * 1024) + p * 1024;
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(m0)), "v"(off[p]), "s"(base)
