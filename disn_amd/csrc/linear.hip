@@ -317,7 +317,9 @@ __device__ __forceinline__ TilePlace tile_place(const TileArgs& a, int block, in
 // rest of the one before; 8 + 8 + 8 bits hold fp32's 24, so the sum is exact) and the six products
 // hh, hm, mh, mm, hl, lh are accumulated in fp32; what is left out (ml, lm, ll) is below 2^-24 of a product, as an
 // FMA's rounding is.  Six bf16 MFMAs take 6/16 of the time of one fp32 MFMA of the same size.  Infinities,
-// NaN and intermediate overflow cannot be cut; a tile whose sums are not all finite is computed again by plain FMAs.
+// NaN and intermediate overflow cannot be cut; a tile whose sums are not all finite is computed again by fp32 MFMAs.
+// Neither can values below 2^-109, whose last term's bits lie below bf16's smallest; a tile that met one (an or over the
+// last terms: an instruction for two values, 2 % of the time) looks whether its sums are small enough to notice, and is computed again if so.
 //
 // LDS: an operand along r as [8 r][i][16 bytes] (half a fragment is 512 bytes in one piece; 128 bytes between the 8-r
 // blocks put the lanes that store a row on different banks); an operand across r as [r][i] with 64 bytes between rows,
@@ -387,7 +389,8 @@ struct Operand {
     }
     if (!ACROSS) first += KT;
   }
-  __device__ __forceinline__ void store(char* lds, int slot, bool shifted) const {
+  // lost: the bits of every last term are or-ed into it; below 2^-109 some lie in its lower half, which bf16 cannot hold
+  __device__ __forceinline__ void store(char* lds, int slot, bool shifted, uint32_t& lost) const {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int t = threadIdx.x + q * THREADS, line = t / PER_LINE, c = t % PER_LINE * V;
@@ -411,6 +414,10 @@ struct Operand {
           for (int i = 0; i < 4; ++i) rest[i] -= (float)term[i];
         }
         __builtin_memcpy(__builtin_assume_aligned(dst + p * PLANE, 8), term, 8);
+        if (p + 2 == P) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) lost |= __builtin_bit_cast(uint32_t, rest[i]);
+        }
       }
     }
   }
@@ -431,34 +438,85 @@ struct Operand {
   }
 };
 
-// a tile of fp32 by plain multiply-adds, eight rows of a column at a time
-__device__ __forceinline__ void fma_tile(const TileArgs& a, bool a_across, bool b_across, int bm, int bn, int threads, int i0, int j0, int split,
-                                      int64_t k0, int have) {
-  const int64_t ai = a_across ? 1 : a.lda, ar = a_across ? a.lda : 1, bj = b_across ? 1 : a.ldb, br = b_across ? a.ldb : 1;
-  for (int t = threadIdx.x; t < bm / 8 * bn; t += threads) {
-    const int i = i0 + t / bn * 8, j = j0 + t % bn;
-    if (i >= a.M || j >= a.N) continue;
-    const float* pa = (const float*)a.A + k0 * ar;
-    const float* pb = (const float*)a.B + j * bj + k0 * br;
-    float s[8];
-    int64_t row[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      s[q] = 0.0f;
-      row[q] = min(i + q, a.M - 1) * ai;
-    }
-    for (int k = 0; k < have; ++k) {
-      const float b = pb[k * br];
-#pragma unroll
-      for (int q = 0; q < 8; ++q) s[q] = fmaf(pa[row[q] + k * ar], b, s[q]);
-    }
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      if (i + q >= a.M) break;
-      if (a.splits > 1) a.part[((size_t)split * a.M + i + q) * a.N + j] = s[q];
-      else finish_one<float>(a.e, i + q, j, s[q]);
+// The largest absolute value of n (<= WIDTH) lines' r values k0 .. k0 + have - 1, for every thread; lds: a float a wave
+template <bool ACROSS, int WIDTH, int THREADS>
+__device__ __forceinline__ float panel_max(const float* p, int64_t ld, int line, int n, int64_t k0, int have, float* lds) {
+  p += ACROSS ? k0 * ld + line : line * ld + k0;
+  // 16 bytes a thread of a run of contiguous values; the last piece of a run lies over the one before it
+  constexpr int PER = ACROSS ? WIDTH / 4 : 64;
+  const int run = ACROSS ? n : have, runs = ACROSS ? have : n;
+  float most = 0.0f;
+  for (int c0 = 0; c0 < run; c0 += PER * 4) {
+    const int c = c0 + (int)threadIdx.x % PER * 4, at = min(c, max(run - 4, 0));
+#pragma unroll 8
+    for (int t = threadIdx.x / PER; t < runs; t += THREADS / PER) {
+      Vec<float> v;
+      if (run >= 4) v = load_vec(p + t * ld + at);
+      else v = load_vec(p + t * ld, run, 0);
+      most = fmaxf(fmaxf(most, fmaxf(fabsf(v.v[0]), fabsf(v.v[1]))), fmaxf(fabsf(v.v[2]), fabsf(v.v[3])));
     }
   }
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) most = fmaxf(most, __shfl_xor(most, m, 64));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = most;
+  __syncthreads();
+  for (int w = 0; w < THREADS / 64; ++w) most = fmaxf(most, lds[w]);
+  return most;
+}
+
+// r = r0 .. r0 + 3 (those below K) of line i (clamped to the matrix by the caller)
+template <typename T, bool ACROSS, bool FULL>
+__device__ __forceinline__ floatx4 load_4r(const void* p_, int64_t ld, int i, int r0, int K) {
+  const T* p = (const T*)p_;
+  floatx4 v;
+  if constexpr (!ACROSS && FULL) {
+    T t[4];
+    __builtin_memcpy(t, p + i * ld + r0, sizeof t);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (float)t[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool in = FULL || r0 + e < K;
+      const int r = in ? r0 + e : 0;
+      const float x = (float)p[ACROSS ? r * ld + i : i * ld + r];
+      v[e] = in ? x : 0.0f;
+    }
+  }
+  return v;
+}
+
+// a wave's sums by fp32 matrix instructions on operands straight from memory, 8 r values a step
+template <bool A_ACROSS, bool B_ACROSS, int MB, int NB>
+__device__ __forceinline__ void fp32_sums(const TileArgs& a, int iw, int jw, int64_t k0, int have, floatx16 (&acc)[MB][NB]) {
+  const int idx = threadIdx.x & 31, half = 4 * ((threadIdx.x & 63) >> 5);
+  const float* pa = (const float*)a.A + (A_ACROSS ? k0 * a.lda : k0);
+  const float* pb = (const float*)a.B + (B_ACROSS ? k0 * a.ldb : k0);
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int g = 0; g < 16; ++g) acc[m][n][g] = 0.0f;
+  auto step = [&](int r, auto full) {
+    constexpr bool FULL = decltype(full)::value;
+    floatx4 va[MB], vb[NB];
+#pragma unroll
+    for (int m = 0; m < MB; ++m) va[m] = load_4r<float, A_ACROSS, FULL>(pa, a.lda, min(iw + m * 32 + idx, a.M - 1), r + half, have);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) vb[n] = load_4r<float, B_ACROSS, FULL>(pb, a.ldb, min(jw + n * 32 + idx, a.N - 1), r + half, have);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(va[m][e], vb[n][e], acc[m][n], 0, 0, 0);
+  };
+  int r = 0;
+#pragma unroll 1
+  for (; r + 8 <= have; r += 8) step(r, std::true_type());
+  if (r < have) step(r, std::false_type());
 }
 
 template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int DEPTH>
@@ -484,6 +542,7 @@ __device__ __forceinline__ void tile32(const TileArgs& a, int block, char* lds) 
 
   OpA A;
   OpB B;
+  uint32_t lost = 0;
   A.init((const T*)a.A, a.lda, i0, a.M, k0);
   B.init((const T*)a.B, a.ldb, j0, a.N, k0);
   auto multiply = [&](int buffer) {
@@ -531,8 +590,8 @@ __device__ __forceinline__ void tile32(const TileArgs& a, int block, char* lds) 
     multiply(buffer);
     if (WHOLE || s + 1 < stages) {
       const bool w = WHOLE || s + 1 < whole;
-      A.store(lds + (1 - buffer) * BUF, slot, w && a_edge);
-      B.store(lds + (1 - buffer) * BUF + OpA::BYTES, slot, w && b_edge);
+      A.store(lds + (1 - buffer) * BUF, slot, w && a_edge, lost);
+      B.store(lds + (1 - buffer) * BUF + OpA::BYTES, slot, w && b_edge, lost);
     }
     if (WHOLE) {
       A.template fetch<true>(slot, KT);
@@ -541,17 +600,19 @@ __device__ __forceinline__ void tile32(const TileArgs& a, int block, char* lds) 
       fetch(slot, s + 1 + DEPTH);
     }
     if (WHOLE) {
-      // the cutting of stage s + 1 runs between the matrix instructions of stage s
+      // the cutting of stage s + 1 runs between the matrix instructions of stage s, so many of its instructions behind each
+      // (100000 x 1984 x 512, W across: 6 984 us, 4 969; along: 6 947, 5 926, 4 946; 16384 x 512 x 512 in 128-wide tiles: 6 55.5, 4 57)
+      constexpr int BETWEEN = BM == 128 ? 6 : B_ACROSS ? 4 : 5;
 #pragma unroll
       for (int i = 0; i < MB * NB * 6; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x2, 6, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, BETWEEN, 0);
       }
     }
   };
   fetch(0, 0);
-  A.store(lds, 0, whole > 0 && a_edge);
-  B.store(lds + OpA::BYTES, 0, whole > 0 && b_edge);
+  A.store(lds, 0, whole > 0 && a_edge, lost);
+  B.store(lds + OpA::BYTES, 0, whole > 0 && b_edge, lost);
 #pragma unroll
   for (int d = 1; d <= DEPTH; ++d) fetch(d % DEPTH, d);
   int s = 0;
@@ -572,10 +633,22 @@ __device__ __forceinline__ void tile32(const TileArgs& a, int block, char* lds) 
       for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int g = 0; g < 16; ++g) bad |= !(fabsf(acc[m][n][g]) <= 3.4028235e38f);
-    if (__syncthreads_or(bad)) {
-      fma_tile(a, A_ACROSS, B_ACROSS, BM, BN, THREADS, i0, j0, split, k0, have);
-      return;
+    bool again = __syncthreads_or(bad || (lost & 0xffff));
+    if (again && !__syncthreads_or(bad)) {
+      // Bits were lost, at most 2^-134 of a value.  Does a sum notice, is it below 2^24 times what all of its products may
+      // have lost?  A sum of 0 (an empty row) is left at 0 where that is below 2^-100.
+      const float most = panel_max<A_ACROSS, BM, THREADS>((const float*)a.A, a.lda, i0, min(a.M - i0, BM), k0, have, (float*)lds) +
+                         panel_max<B_ACROSS, BN, THREADS>((const float*)a.B, a.ldb, j0, min(a.N - j0, BN), k0, have, (float*)lds);
+      const float least = most * (float)have * 0x1p-109f;
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int g = 0; g < 16; ++g) bad |= fabsf(acc[m][n][g]) < least && (acc[m][n][g] != 0.0f || least > 0x1p-76f);
+      again = __syncthreads_or(bad);
     }
+    if (again) fp32_sums<A_ACROSS, B_ACROSS, MB, NB>(a, i0 + wi, j0 + wj, k0, have, acc);
   }
   tile_end<T, MB, NB, WM * WN>(a, split, i0 + wi, j0 + wj, acc, (float*)lds);
 }
@@ -853,33 +926,12 @@ struct SmallArgs {
 };
 constexpr int SMALL_WAVES = 8;
 
-// r = r0 .. r0 + 3 (those below K) of line i (clamped to the matrix by the caller)
-template <typename T, bool ACROSS, bool FULL>
-__device__ __forceinline__ floatx4 small_load(const void* p_, int64_t ld, int i, int r0, int K) {
-  const T* p = (const T*)p_;
-  floatx4 v;
-  if constexpr (!ACROSS && FULL) {
-    T t[4];
-    __builtin_memcpy(t, p + i * ld + r0, sizeof t);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (float)t[e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool in = FULL || r0 + e < K;
-      const int r = in ? r0 + e : 0;
-      const float x = (float)p[ACROSS ? r * ld + i : i * ld + r];
-      v[e] = in ? x : 0.0f;
-    }
-  }
-  return v;
-}
 template <typename T, bool ACROSS, bool GATED, bool FULL>
 __device__ __forceinline__ floatx4 small_operand(const SmallOperand& o, int i, int r0, int K, int act) {
-  floatx4 v = small_load<T, ACROSS, FULL>(o.p, o.ld, i, r0, K);
+  floatx4 v = load_4r<T, ACROSS, FULL>(o.p, o.ld, i, r0, K);
   if constexpr (GATED) {
     if (act != DISN_ACT_NONE) {
-      const floatx4 z = small_load<T, ACROSS, FULL>(o.gate, o.ldg, i, r0, K);
+      const floatx4 z = load_4r<T, ACROSS, FULL>(o.gate, o.ldg, i, r0, K);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] *= FULL || r0 + e < K ? slope(z[e], act) : 1.0f;
     }

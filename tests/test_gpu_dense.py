@@ -259,6 +259,35 @@ def test_linear_float32_range(ctx, m, k, n):
     assert (y[:, 0] == float("inf")).all() and (y[:, 1] == float("-inf")).all()
 
 
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("xs,ws", [(-120, 100), (-132, 118), (-145, 120), (118, -132), (-119, 0), (-60, -62)])
+@pytest.mark.parametrize("m,k,n", [(20, 40, 30), (4, 1100, 1000), (300, 700, 800), (2000, 512, 515), (3000, 900, 1100), (40000, 200, 260)])
+def test_linear_float32_smallest_values(ctx, m, k, n, xs, ws, layout):
+    """values whose last bits lie next to the smallest of float32, or below those of a narrower type"""
+    g = gen(m, k, n, xs, ws)
+    x = (torch.randn(m, k, generator=g, device=DEV).double() * 2.0 ** xs).float()
+    w = (torch.randn(k, n, generator=g, device=DEV).double() * 2.0 ** ws).float()
+    # (k + 4) roundings as everywhere, and six partial sums that may each be rounded to steps of 2^-149 a term
+    bound = 2 * (k + 4) * E * (x.double().abs() @ w.double().abs()) + 6 * (k + 4) * 2.0 ** -149
+    within(ctx.linear(x, weight(w, layout)), x.double() @ w.double(), bound)
+    dy = x.repeat(1, n // k + 1)[:, :n].contiguous()
+    dx, _, _ = ctx.linear_backward(dy, x, weight(w, layout))
+    within(dx, dy.double() @ w.double().t(), 2 * (n + 4) * E * (dy.double().abs() @ w.double().abs().t()) + 6 * (n + 4) * 2.0 ** -149)
+
+
+@pytest.mark.parametrize("m,k,n", [(300, 700, 800), (3000, 900, 1100), (40000, 200, 260)])
+def test_linear_float32_small_among_others(ctx, m, k, n):
+    """rows of small values, rows of zeros and ordinary rows in one matrix"""
+    g = gen(m, k, n, 8)
+    x, w = torch.randn(m, k, generator=g, device=DEV), torch.randn(k, n, generator=g, device=DEV)
+    x[::3] *= 2.0 ** -122
+    x[1::6] = 0.0
+    x[2::3, ::5] *= 2.0 ** -125
+    y = ctx.linear(x, w)
+    within(y, x.double() @ w.double(), 2 * (k + 4) * E * (x.double().abs() @ w.double().abs()) + 6 * (k + 4) * 2.0 ** -149)
+    assert (y[1::6] == 0).all()
+
+
 def norm_inputs(rows, d, kind, seed):
     g = gen(rows, d, kind, seed)
     x = (torch.randn(rows, d, generator=g, device=DEV) * (0.2 + 3 * torch.rand(rows, 1, generator=g, device=DEV)) +
