@@ -309,7 +309,8 @@ class Context:
     def linear(self, x, w, bias=None, residual=None, act="none", want_pre=False, out=None):
         """act(x @ w + bias) + residual (disn_linear).  x: [..., k]; w: [k, n] by rows, or the .t() of an [n, k] matrix;
         bias: [n]; residual: [..., n]; act: none, relu, gelu (erf), silu.  want_pre: -> (y, x @ w + bias), the second for
-        linear_backward.  out: a tensor for y, which may be the residual itself but overlaps no other argument."""
+        linear_backward.  out: a tensor for y, which may be the residual itself but overlaps no other argument.
+        k and n go up to 4194304, the rows up to 2^30."""
         if self._elsewhere():
             with torch.cuda.device(self.device):
                 return self.linear(x, w, bias, residual, act, want_pre, out)

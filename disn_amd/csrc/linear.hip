@@ -1239,7 +1239,8 @@ struct Plan {
 };
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 // k_tile16 reads 16-byte pieces at 32-bit offsets from a tile's first value
-bool tile16_ready(const void* p, int64_t ld) { return dense_aligned(p, 16) && ld % 8 == 0 && ld <= 1 << 22; }
+bool tile16_ready(const void* p, int64_t ld) { return dense_aligned(p, 16) && ld % 8 == 0 && ld <= DISN_LINEAR_MAX; }
+static_assert(255ll * DISN_LINEAR_MAX * 2 + 64 < 1ll << 32, "offsets of the 256 lines of a tile");
 size_t pack_bytes(int64_t rows, int64_t cols) { return align256((size_t)rows * ((cols + 7) / 8 * 8) * 2); }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -1515,13 +1516,17 @@ int run_product(DisnCtx* ctx, Product q, Plan p, char* ws, hipStream_t stream) {
 }
 
 // ---- host: arguments -----------------------------------------------------------------------------------------------------
+// n and k are bounded by the 32-bit offsets of a tile's operands (tile16_ready; a copy's rows are as long as n or k) and by
+// the grids of k_rows_along and k_sum_partials
+bool linear_size_ok(int64_t v) { return v >= 0 && v <= DISN_LINEAR_MAX; }
 int check_linear(DisnCtx* ctx, const DisnLinear* a) {
   const char* f = "disn_linear";
   if (!a) return disn_fail(ctx, DISN_E_ARG, "%s: null arguments", f);
   if (!dense_type_ok(a->type) || a->act < DISN_ACT_NONE || a->act > DISN_ACT_SILU || a->w_nk < 0 || a->w_nk > 1 || a->reserved)
     return disn_fail(ctx, DISN_E_ARG, "%s: bad type %d, act %d, w_nk %d or reserved field", f, a->type, a->act, a->w_nk);
-  if (!dense_size_ok(a->m) || !dense_size_ok(a->n) || !dense_size_ok(a->k))
-    return disn_fail(ctx, DISN_E_ARG, "%s: sizes %lld, %lld, %lld", f, (long long)a->m, (long long)a->n, (long long)a->k);
+  if (!dense_size_ok(a->m) || !linear_size_ok(a->n) || !linear_size_ok(a->k))
+    return disn_fail(ctx, DISN_E_ARG, "%s: sizes m %lld, n %lld, k %lld (n and k up to %d)", f, (long long)a->m, (long long)a->n,
+                     (long long)a->k, DISN_LINEAR_MAX);
   const size_t s = dense_type_size(a->type);
   if (a->m == 0 || a->n == 0) return DISN_OK;
   if (!dense_matrix_ok(a->x, a->m, a->k, a->ldx, s, true) ||
@@ -1538,8 +1543,9 @@ int check_linear_grad(DisnCtx* ctx, const DisnLinearGrad* a) {
   if (!a) return disn_fail(ctx, DISN_E_ARG, "%s: null arguments", f);
   if (!dense_type_ok(a->type) || a->act < DISN_ACT_NONE || a->act > DISN_ACT_SILU || a->w_nk < 0 || a->w_nk > 1 || a->reserved)
     return disn_fail(ctx, DISN_E_ARG, "%s: bad type %d, act %d, w_nk %d or reserved field", f, a->type, a->act, a->w_nk);
-  if (!dense_size_ok(a->m) || !dense_size_ok(a->n) || !dense_size_ok(a->k))
-    return disn_fail(ctx, DISN_E_ARG, "%s: sizes %lld, %lld, %lld", f, (long long)a->m, (long long)a->n, (long long)a->k);
+  if (!dense_size_ok(a->m) || !linear_size_ok(a->n) || !linear_size_ok(a->k))
+    return disn_fail(ctx, DISN_E_ARG, "%s: sizes m %lld, n %lld, k %lld (n and k up to %d)", f, (long long)a->m, (long long)a->n,
+                     (long long)a->k, DISN_LINEAR_MAX);
   const size_t s = dense_type_size(a->type);
   const int64_t wr = a->w_nk ? a->n : a->k, wc = a->w_nk ? a->k : a->n;
   if ((a->act == DISN_ACT_NONE) != !a->pre && a->m && a->n)

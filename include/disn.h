@@ -182,8 +182,9 @@ int disn_vgg_forward(DisnCtx* ctx, int slot, const float* img, int img_h, int im
  * models/posenet_old.py:104-142, and has no norm): for decoders of other widths, residual blocks and the training of
  * either.  Common rules:
  *  - every tensor of a call has the same type; statistics, sums and partial results are fp32, a result is rounded once
- *  - matrices are rows of contiguous values, `ld*` values apart (ld >= the row's length; inputs may have ld = 0: one
- *    row for all).  Any base address that fits the type, any size and any ld are allowed; sizes up to 2^30
+ *  - matrices are rows of contiguous values, `ld*` values apart (ld >= the row's length, up to 2^31; inputs may have
+ *    ld = 0: one row for all).  Any base address that fits the type is allowed.  Up to 2^30 rows (m, rows); n and k of
+ *    a dense layer up to DISN_LINEAR_MAX
  *  - a size of zero is fine: an empty output is not written, a sum over nothing is 0
  *  - an output must not overlap any other argument.  One exception: y of disn_linear may be the residual itself
  *    (same address and ld)
@@ -195,6 +196,7 @@ int disn_vgg_forward(DisnCtx* ctx, int slot, const float* img, int img_h, int im
 #define DISN_F32 0
 #define DISN_BF16 1
 #define DISN_F16 2
+#define DISN_LINEAR_MAX 4194304
 #define DISN_ACT_NONE 0
 #define DISN_ACT_RELU 1
 #define DISN_ACT_GELU 2 /* z (1 + erf(z / sqrt 2)) / 2 */

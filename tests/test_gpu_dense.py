@@ -259,6 +259,32 @@ def test_linear_float32_range(ctx, m, k, n):
     assert (y[:, 0] == float("inf")).all() and (y[:, 1] == float("-inf")).all()
 
 
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_linear_longest_rows(ctx, kind):
+    """sums over the largest k, on and off 16-byte boundaries, and rows of the largest n"""
+    top = 1 << 22
+    g = gen(kind, 9)
+    x, w = ints(g, kind, 130, top, top=1), ints(g, kind, 132, top, top=1)
+    want = torch.zeros(130, 132, dtype=torch.float64, device=DEV)
+    for part in range(0, top, top // 8):                   # whole numbers up to 2^22: every order of the sums is exact
+        c = slice(part, part + top // 8)
+        want += x[:, c].double() @ w[:, c].double().t()
+    same(ctx.linear(x, w.t()), want)
+    off = torch.empty(130 * top + 1, dtype=x.dtype, device=DEV)[1:].view(130, top)
+    off.copy_(x)
+    same(ctx.linear(off, w.t()), want)
+    del off
+    dx, dw, db = ctx.linear_backward(x, w[0].repeat(130, 1)[:, :3].contiguous(), w[:3])   # n = top
+    same(db, x.double().sum(0))
+    del db, dw
+    assert dx.shape == (130, 3)
+    same(dx, want[:, :3])
+    v = ints(g, kind, 24, top, top=1)
+    same(ctx.linear(x[:40, :24].contiguous(), v)[:, -300:], x[:40, :24].double() @ v[:, -300:].double())
+    y = ctx.linear(x[:2, :24].contiguous(), v[:, 1:].contiguous())
+    same(y, x[:2, :24].double() @ v[:, 1:].double())
+
+
 @pytest.mark.parametrize("layout", ["kn", "nk"])
 @pytest.mark.parametrize("xs,ws", [(-120, 100), (-132, 118), (-145, 120), (118, -132), (-119, 0), (-60, -62)])
 @pytest.mark.parametrize("m,k,n", [(20, 40, 30), (4, 1100, 1000), (300, 700, 800), (2000, 512, 515), (3000, 900, 1100), (40000, 200, 260)])
@@ -562,6 +588,23 @@ def test_refusals_of_tensors(ctx):
     assert ctx.linear(buf[:, :8], w, out=buf[:, 8:14]).sum() == 4 * 6 * 8     # other columns of the same rows: no overlap
     with pytest.raises(api.DisnError, match="overlaps"):
         ctx.layer_norm(x, out=x)
+
+
+def test_refusals_of_sizes(ctx):
+    import ctypes
+    lib, h, n = _lib.load(), ctx._h, ctypes.c_size_t()
+    p = torch.ones(64, device=DEV).data_ptr()
+    top = 1 << 22
+    for big in (dict(k=top + 1, ldx=top + 1), dict(n=top + 1, ldw=top + 1, ldy=top + 1), dict(m=(1 << 30) + 1)):
+        a = _lib.DisnLinear(1, 0, 0, 0, 4, 8, 8, p, 64, p, 64, None, None, 0, p, 64, None, 0)
+        b = _lib.DisnLinearGrad(1, 0, 0, 0, 4, 8, 8, p, 64, p, 64, p, 64, None, 0, None, 0, None, 0, p)
+        for key, v in big.items():
+            setattr(a, key, v)
+            setattr(b, key.replace("ldy", "lddy"), v)
+        assert lib.disn_linear_workspace(h, ctypes.byref(a), ctypes.byref(n)) == -1 and b"sizes" in lib.disn_last_error(h)
+        assert lib.disn_linear(h, ctypes.byref(a), None, 0, None) == -1 and b"sizes" in lib.disn_last_error(h)
+        assert lib.disn_linear_backward_workspace(h, ctypes.byref(b), ctypes.byref(n)) == -1 and b"sizes" in lib.disn_last_error(h)
+        assert lib.disn_linear_backward(h, ctypes.byref(b), None, 0, None) == -1 and b"sizes" in lib.disn_last_error(h)
 
 
 def test_refusals_of_the_c_abi(ctx):
