@@ -7,10 +7,15 @@
 //
 // Both are bound by memory: every value is read once and written once.  A group of G threads holds a whole row in
 // registers, E values a thread in 16-byte pieces, so the variance is the sum of squared distances from the mean that
-// is already known (not a difference of two large sums) and costs no second read.  G = 16 / 64: rows inside a wave
-// (no barrier, sums by lane exchange), 256 / 1024: a row per workgroup.  The backward pass walks over rows with a
+// is already known (not a difference of two large sums) and costs no second read.  G up to 64: rows inside a wave
+// (no barrier, sums by lane exchange), 256 / 512: a row per workgroup.  The backward pass walks over rows with a
 // fixed set of workgroups; a thread meets the same columns in every row and sums their dg, db in registers; the
-// workgroups' sums are added in order by a second kernel.
+// workgroups' sums are added in order by a second kernel.  Few waves fit beside these registers, so each reads its next
+// row while it works on the present one (us without / with, 300 MB of bf16 rows: d = 768 343 / 167, 1024 276 / 168,
+// 4096 300 / 189); so does the forward pass of the longest rows (d = 5000 168 / 127).
+// Measured: 262144 x 512 bf16 forward 106 us (5.1 TB/s of what is read and written), backward with a residual 194 us (5.5), 5003 x 1537
+// fp32 backward 25 us (3.7).  Rows of 16-bit values that start at odd places are slower, 16 bytes of them at a time cost the
+// memory pipe two accesses: 300 MB in rows of 1031 forward 198 us, backward 325; of 1024 114 and 176.
 #include "dense.h"
 
 namespace {
@@ -105,8 +110,8 @@ struct Row {
 };
 
 template <typename T, int G, int E, Ends ENDS>
-__global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm(NormArgs a) {
-  constexpr int N = Vec<T>::N, P = E / N, B = G < 256 ? 256 : G;
+__global__ __launch_bounds__(G <= 64 ? 256 : G) void k_layer_norm(NormArgs a) {
+  constexpr int N = Vec<T>::N, P = E / N, B = G <= 64 ? 256 : G;
   __shared__ float lds[2][16];
   const int t = threadIdx.x % G, d = a.d;
   const Row<T, G, E, ENDS> ends(t, d);
@@ -123,9 +128,20 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm(NormArgs a) {
     }
   }
   const float inv = 1.0f / (float)d;
-  for (int64_t row = (int64_t)blockIdx.x * (B / G) + threadIdx.x / G; row < a.rows; row += (int64_t)gridDim.x * (B / G)) {
+  constexpr bool AHEAD = G == 512;   // the next row is read early
+  const int64_t step = (int64_t)gridDim.x * (B / G);
+  int64_t row = (int64_t)blockIdx.x * (B / G) + threadIdx.x / G;
+  Vec<T> next[P];
+  if (AHEAD) ends.load((const T*)a.x + row * a.ldx, next);   // (no more workgroups than rows)
+  for (; row < a.rows; row += step) {
     Vec<T> xv[P];
-    ends.load((const T*)a.x + row * a.ldx, xv);
+    if (AHEAD) {
+#pragma unroll
+      for (int p = 0; p < P; ++p) xv[p] = next[p];
+      ends.load((const T*)a.x + min(row + step, a.rows - 1) * a.ldx, next);
+    } else {
+      ends.load((const T*)a.x + row * a.ldx, xv);
+    }
     ends.settle(xv);
     float x[E];
     widen<T, E>(xv, x);
@@ -162,8 +178,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm(NormArgs a) {
 }
 
 template <typename T, int G, int E, Ends ENDS>
-__global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm_backward(NormArgs a) {
-  constexpr int N = Vec<T>::N, P = E / N, B = G < 256 ? 256 : G;
+__global__ __launch_bounds__(G <= 64 ? 256 : G) void k_layer_norm_backward(NormArgs a) {
+  constexpr int N = Vec<T>::N, P = E / N, B = G <= 64 ? 256 : G;
   __shared__ float lds[2][16];
   const int t = threadIdx.x % G, d = a.d;
   const Row<T, G, E, ENDS> ends(t, d);
@@ -178,12 +194,24 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm_backward(NormA
 #pragma unroll
   for (int i = 0; i < E; ++i) dg[i] = db[i] = 0.0f;
   const float inv = 1.0f / (float)d;
-  for (int64_t row = (int64_t)blockIdx.x * (B / G) + threadIdx.x / G; row < a.rows; row += (int64_t)gridDim.x * (B / G)) {
+  Vec<T> next_x[P], next_g[P], next_r[P];
+  float next_mean, next_rstd;
+  auto fetch = [&](int64_t row) {
+    row = min(row, a.rows - 1);
+    ends.load((const T*)a.x + row * a.ldx, next_x);
+    ends.load((const T*)a.dy + row * a.lddy, next_g);
+    if (a.y && a.residual) ends.load((const T*)a.residual + row * a.ldr, next_r);
+    next_mean = a.mean_in[row], next_rstd = a.rstd_in[row];
+  };
+  const int64_t step = (int64_t)gridDim.x * (B / G);
+  int64_t row = (int64_t)blockIdx.x * (B / G) + threadIdx.x / G;
+  if (a.rows > 0) fetch(row);
+  for (; row < a.rows; row += step) {
     Vec<T> xv[P], gv[P], rv[P];
-    ends.load((const T*)a.x + row * a.ldx, xv);
-    ends.load((const T*)a.dy + row * a.lddy, gv);
-    if (a.y && a.residual) ends.load((const T*)a.residual + row * a.ldr, rv);
-    const float mean = a.mean_in[row], rstd = a.rstd_in[row];
+#pragma unroll
+    for (int p = 0; p < P; ++p) xv[p] = next_x[p], gv[p] = next_g[p], rv[p] = next_r[p];
+    const float mean = next_mean, rstd = next_rstd;
+    fetch(row + step);
     ends.settle(xv);
     ends.settle(gv);
     if (a.y && a.residual) ends.settle(rv);
@@ -237,6 +265,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm_backward(NormA
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           float s = red[threadIdx.x * E + i];
+#pragma unroll 2   // (all of them ahead are more registers than the rows need)
           for (int k = 1; k < K; ++k) s += red[(k * G + threadIdx.x) * E + i];
           v[i] = s;
         }
@@ -260,35 +289,37 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_layer_norm_backward(NormA
   }
 }
 
-// group size and values per thread for a row of d values.  Small rows share a wave; up to 1024 values a wave
-// holds a row without barriers; the row is spread wider before a thread holds more than 16 values.
+// Group size and values per thread for a row of d values: the smallest group that holds it, 8 values a thread, up to a
+// wave (lanes without values cost time: 16-bit rows of 40 in groups of 8 / 16 136 / 212 us, rows of 200 in groups of 32 / 64
+// 130 / 183); 16 a thread before a row is spread over more waves.
 struct NormShape {
   int group, per_thread;
 };
 NormShape norm_shape(int64_t d) {
-  if (d <= 128) return {16, 8};
-  if (d <= 512) return {64, 8};
+  if (d <= 512) return {d <= 64 ? 8 : d <= 128 ? 16 : d <= 256 ? 32 : 64, 8};
   if (d <= 1024) return {64, 16};
   if (d <= 2048) return {256, 8};
   if (d <= 4096) return {256, 16};
-  return {1024, 8};
+  return {512, 16};
 }
-// Workgroups of the backward pass: what the chip holds of them at once (more than 8 values a thread take twice the
-// registers), each at least two rows a group, so that the partial sums (2 d floats a workgroup) stay small beside the rows
-// it reads.  Measured in us at 256 / 512 / 768 / 1024 workgroups: 262144 x 512 bf16 473 / 280 / 212 / 181, 5003 x 1536 fp32
-// 38 / 28 / 26 / 27, 4000 x 4096 bf16 64 / 50 / 50 / 65, 60000 x 1024 fp32 156 / 141 / 145 / 153.
-int64_t norm_backward_grid(const NormShape& s, int64_t rows) {
-  const int64_t per = s.group < 256 ? 256 / s.group : 1;
-  const int64_t most = s.group == 1024 ? 256 : s.per_thread > 8 ? 512 : s.group == 256 ? 768 : 1024, want = (rows + per * 2 - 1) / (per * 2);
+int64_t norm_rows_at_once(const NormShape& s) { return s.group <= 64 ? 256 / s.group : 1; }
+// Workgroups of the backward pass: what the chip holds of them at once, each at least two rows a group, so that the partial
+// sums (2 d floats a workgroup) stay small beside the rows it reads.
+// Measured in us at 256 / 512 / 768 / 1024 workgroups, 300 MB of rows: 512 bf16 253 / 170 / 161 / 171 and fp32
+// 244 / 167 / 175 / 176, 1024 bf16 172 / 168 / 181 / 202, 2000 bf16 496 / 270 / 216 / 195 and fp32 270 / 170 / 173 / 183, 1100
+// fp32 432 / 240 / 190 / 174, 3001 bf16 393 / 282 / 323 / 295, 5000 bf16 265 / 274 / 284 / 292.
+int64_t norm_backward_grid(const NormShape& s, int type, int64_t rows) {
+  const int64_t per = norm_rows_at_once(s), want = (rows + per * 2 - 1) / (per * 2);
+  const int64_t most = s.group == 512 ? 256 : s.per_thread > 8 ? 512 : s.group == 256 && type != DISN_F32 ? 1024 : 768;
   return want < 1 ? 1 : want < most ? want : most;
 }
 
 template <typename T, int G, int E>
 void launch_norm(bool backward, const NormArgs& a, int64_t grid, hipStream_t stream) {
-  constexpr int B = G < 256 ? 256 : G;
+  constexpr int B = G <= 64 ? 256 : G;
   const int N = Vec<T>::N;
   const Ends ends = a.d % N == 0 ? WHOLE : a.d > N ? SHIFT : SHORT;
-  if constexpr (G == 16)
+  if constexpr (G == 8)
     if (ends == SHORT) {
       if (backward) k_layer_norm_backward<T, G, E, SHORT><<<(unsigned)grid, B, 0, stream>>>(a);
       else k_layer_norm<T, G, E, SHORT><<<(unsigned)grid, B, 0, stream>>>(a);
@@ -301,12 +332,14 @@ void launch_norm(bool backward, const NormArgs& a, int64_t grid, hipStream_t str
 }
 template <typename T>
 void launch_norm(const NormShape& s, bool backward, const NormArgs& a, int64_t grid, hipStream_t stream) {
-  if (s.group == 16) launch_norm<T, 16, 8>(backward, a, grid, stream);
+  if (s.group == 8) launch_norm<T, 8, 8>(backward, a, grid, stream);
+  else if (s.group == 16) launch_norm<T, 16, 8>(backward, a, grid, stream);
+  else if (s.group == 32) launch_norm<T, 32, 8>(backward, a, grid, stream);
   else if (s.group == 64 && s.per_thread == 8) launch_norm<T, 64, 8>(backward, a, grid, stream);
   else if (s.group == 64) launch_norm<T, 64, 16>(backward, a, grid, stream);
   else if (s.group == 256 && s.per_thread == 8) launch_norm<T, 256, 8>(backward, a, grid, stream);
   else if (s.group == 256) launch_norm<T, 256, 16>(backward, a, grid, stream);
-  else launch_norm<T, 1024, 8>(backward, a, grid, stream);
+  else launch_norm<T, 512, 16>(backward, a, grid, stream);
 }
 
 int check_norm(DisnCtx* ctx, const DisnLayerNorm* a) {
@@ -344,7 +377,7 @@ int check_norm_grad(DisnCtx* ctx, const DisnLayerNormGrad* a) {
 
 size_t norm_grad_workspace(const DisnLayerNormGrad* a) {
   if (!a->dweight && !a->dbias) return 0;
-  const int64_t grid = norm_backward_grid(norm_shape(a->d), a->rows);
+  const int64_t grid = norm_backward_grid(norm_shape(a->d), a->type, a->rows);
   return grid == 1 ? 0 : (size_t)grid * 2 * a->d * sizeof(float);
 }
 
@@ -359,7 +392,7 @@ extern "C" int disn_layer_norm(DisnCtx* ctx, const DisnLayerNorm* a, void* strea
   k.x = a->x, k.weight = a->weight, k.bias = a->bias, k.y = a->y, k.mean = a->mean, k.rstd = a->rstd;
   k.ldx = a->ldx, k.ldy = a->ldy, k.rows = a->rows, k.d = (int)a->d, k.eps = (float)a->eps;
   const NormShape s = norm_shape(a->d);
-  const int64_t per = s.group < 256 ? 256 / s.group : 1, want = (a->rows + per - 1) / per, most = s.group == 1024 ? 512 : 2048;
+  const int64_t per = norm_rows_at_once(s), want = (a->rows + per - 1) / per, most = s.group == 512 ? 512 : 4096;
   dense_dispatch(a->type, [&](auto t) {
     launch_norm<decltype(t)>(s, false, k, want < most ? want : most, (hipStream_t)stream_);
     return 0;
@@ -391,7 +424,7 @@ extern "C" int disn_layer_norm_backward(DisnCtx* ctx, const DisnLayerNormGrad* a
   k.y = a->dx, k.dweight = a->dweight, k.dbias = a->dbias, k.part = (float*)workspace;
   k.ldx = a->ldx, k.lddy = a->lddy, k.ldr = a->ldr, k.ldy = a->lddx, k.rows = a->rows, k.d = (int)a->d;
   const NormShape s = norm_shape(a->d);
-  const int64_t grid = norm_backward_grid(s, a->rows);   // without rows one workgroup writes the empty sums
+  const int64_t grid = norm_backward_grid(s, a->type, a->rows);   // without rows one workgroup writes the empty sums
   dense_dispatch(a->type, [&](auto t) {
     using T = decltype(t);
     launch_norm<T>(s, true, k, grid, stream);
