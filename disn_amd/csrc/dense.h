@@ -70,6 +70,17 @@ __device__ __forceinline__ Vec<T> load_vec(const T* p, int n, int64_t before) {
   }
   return __builtin_bit_cast(Vec<T>, w);
 }
+// what a load from `back` (< N) values further in front gave, without those values; zeros behind
+template <typename T>
+__device__ __forceinline__ Vec<T> shift_vec(const Vec<T>& v, int back) {
+  uint64_t w[2];
+  __builtin_memcpy(w, &v, 16);
+  const int s = back * (8 * (int)sizeof(T));
+  const uint64_t hi = w[1];
+  w[0] = s >= 64 ? hi >> (s & 63) : (w[0] >> s) | ((hi << 1) << (63 - s));
+  w[1] = s >= 64 ? 0 : hi >> s;
+  return __builtin_bit_cast(Vec<T>, w);
+}
 // the first n (n >= N: all) values to p
 template <typename T>
 __device__ __forceinline__ void store_vec(T* p, const Vec<T>& r, int n) {

@@ -6,10 +6,12 @@
 //   dW  r = row                            A = x, B = dz ([k][n]) or A = dz, B = x ([n][k])
 // An operand lies "along" r (its r values are contiguous) or "across" (its i values are, rows of r).
 //
-// Three kernels compute it, chosen by size (plan() below):
+// The kernels that compute it, chosen by size (plan() below):
 //   k_tile16, k_tile32  large products: 128- or 256-wide tiles through LDS on the matrix cores
 //   k_small  products of some microseconds: no LDS tiles, the waves of a workgroup share the sum
 //   k_rows_* at most 4 rows times a large matrix: W streams past at memory speed
+//   k_outer  sums of up to 8 products: C is what takes time to write
+//   k_thin   long sums for a C of up to 8 rows or columns: the wider operand is what takes time to read
 #include "dense.h"
 
 #include <atomic>
@@ -1141,8 +1143,131 @@ __global__ __launch_bounds__(256) void k_rows_along(RowsArgs a) {
   }
 }
 
+// ---- k_outer: sums of up to 8 products ---------------------------------------------------------------------------------
+// (the first layer of three coordinates; gradients of a layer with few outputs or of few rows).  Bound by writing C: a lane
+// keeps its 16 bytes of columns of B and walks over rows, several of them under way.
+// 262144 x 512 results of one product: bf16 49 us (5.5 TB/s), k_small 152; fp32 135 and 186; of three products in fp32, 65536
+// rows 36 and 45.  In 16 bits more products are faster in tiles (65536 x 512 of three 24 us, here 37; but 262144 x 64 here 25,
+// k_small 35).
+struct OuterArgs {
+  const void *A, *B;
+  int64_t ai, ar, bj, br;   // distances along i, j and r
+  int64_t M, rows_per;
+  int N, K, lanes, groups;
+  Epilogue e;
+};
+constexpr int THIN = 8;     // the longest sum of k_outer, the widest narrow operand of k_thin
+template <typename T, int KR>
+__global__ __launch_bounds__(256) void k_outer(OuterArgs a) {
+  constexpr int V = Vec<T>::N, U = 4;
+  const int L = a.lanes, sub = threadIdx.x % L, line = threadIdx.x / L, lines = 256 / L;
+  const int group = blockIdx.x % a.groups;
+  const int64_t i0 = (int64_t)(blockIdx.x / a.groups) * a.rows_per, i1 = min(a.M, i0 + a.rows_per);
+  const int col = (group * L + sub) * V, n = a.N - col;
+  if (n <= 0) return;
+  float b[KR][V];
+#pragma unroll
+  for (int k = 0; k < KR; ++k)
+#pragma unroll
+    for (int v = 0; v < V; ++v) b[k][v] = k < a.K && v < n ? (float)((const T*)a.B)[(col + v) * a.bj + k * a.br] : 0.0f;
+  const Vec<T> bias = bias_vec<T>(a.e, col, n);
+  for (int64_t i = i0 + line; i < i1; i += U * lines) {
+    float x[U][KR];
+    Vec<T> res[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = min(i + u * lines, i1 - 1);
+#pragma unroll
+      for (int k = 0; k < KR; ++k) x[u][k] = k < a.K ? (float)((const T*)a.A)[row * a.ai + k * a.ar] : 0.0f;
+      res[u] = residual_vec<T>(a.e, row, col, n);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = i + u * lines;
+      if (row >= i1) break;
+      float z[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        z[v] = x[u][0] * b[0][v];
+#pragma unroll
+        for (int k = 1; k < KR; ++k)
+          if (k < a.K) z[v] = fmaf(x[u][k], b[k][v], z[v]);
+      }
+      finish_vec<T>(a.e, (T*)a.e.out + row * a.e.ldo + col, (T*)a.e.pre + row * a.e.ldp + col, z, n, bias, res[u]);
+    }
+  }
+}
+
+// ---- k_thin: long sums of a wide and a narrow operand, both across r -----------------------------------------------------
+// (the weight's gradient of a layer with few outputs or few inputs).  Bound by reading the wide operand: a lane owns 16 bytes
+// of its columns and sums their products with each of up to 8 columns of the narrow one; parts of r become partial sums.
+// Weight's gradient over 262144 rows of 512 inputs and one output, fp32: 104 us (5.2 TB/s), 356 in tiles.  fp32 only: in 16
+// bits the tiles are as fast (65536 x 512, one output: 20 us both).
+struct ThinArgs {
+  const float *wide, *narrow;
+  int64_t ldw, ldn, K, rows_per;
+  int D, S, lanes, groups;
+  int64_t od, os, size;   // places in C of the wide operand's columns, the narrow one's, and of all
+  float* part;
+};
+template <int SR>
+__global__ __launch_bounds__(256) void k_thin(ThinArgs a) {
+  constexpr int V = 4, U = 8;
+  __shared__ float red[4][64 * V];
+  const int L = a.lanes, sub = threadIdx.x % L, line = threadIdx.x / L, lines = 256 / L, wave = threadIdx.x >> 6;
+  const int group = blockIdx.x % a.groups;
+  const int64_t split = blockIdx.x / a.groups, r0 = split * a.rows_per, r1 = min(a.K, r0 + a.rows_per);
+  const int col = (group * L + sub) * V, back = col < a.D && col + V > a.D ? col + V - a.D : 0;
+  const float* w = a.wide + (col < a.D ? col - back : 0);   // lanes behind the last column: the first ones, not stored
+  const bool ragged = (group + 1) * L * V > a.D;
+  float acc[SR][V];
+#pragma unroll
+  for (int s = 0; s < SR; ++s)
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[s][v] = 0.0f;
+  for (int64_t r = r0 + line; r < r1; r += U * lines) {
+    Vec<float> x[U];
+    float t[U][SR];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = min(r + u * lines, r1 - 1);
+      x[u] = load_vec(w + row * a.ldw);
+#pragma unroll
+      for (int s = 0; s < SR; ++s) t[u][s] = s < a.S ? a.narrow[row * a.ldn + s] : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (r + u * lines >= r1) break;
+      if (ragged) x[u] = shift_vec(x[u], back);
+#pragma unroll
+      for (int s = 0; s < SR; ++s)
+        if (s < a.S) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) acc[s][v] = fmaf(x[u].v[v], t[u][s], acc[s][v]);
+        }
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < SR; ++s) {
+    if (s >= a.S) break;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      for (int d = L; d < 64; d <<= 1) acc[s][v] += __shfl_xor(acc[s][v], d, 64);
+      if ((threadIdx.x & 63) < L) red[wave][sub * V + v] = acc[s][v];
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < L * V; t += 256) {
+      const int j = group * L * V + t;
+      if (j < a.D) a.part[split * a.size + j * a.od + s * a.os] = (red[0][t] + red[1][t]) + (red[2][t] + red[3][t]);
+    }
+    __syncthreads();
+  }
+}
+
 // ---- dz = dy act'(pre) and partial column sums of it -------------------------------------------------------------------
-// A lane owns 16 bytes of columns; rows narrower than a wave put several rows into it.
+// A lane owns 16 bytes of columns (SINGLE: one, for rows of less than 16 bytes); rows narrower than a wave put several of them
+// into it.  Four rows are under way.  Bound by memory: 65536 x 512 bf16 relu 41 us, 4.9 TB/s
+// of the three matrices.
 struct GateArgs {
   const void *dy, *pre;
   void* dz;          // null: only the sums
@@ -1150,76 +1275,73 @@ struct GateArgs {
   int64_t lddy, ldp, ldz, M, rows_per;
   int N, lanes, groups, act;
 };
-template <typename T>
+template <typename T, bool SINGLE>
 __global__ __launch_bounds__(256) void k_gate(GateArgs a) {
-  constexpr int V = Vec<T>::N;
-  __shared__ float red[256 * V];
+  constexpr int V = SINGLE ? 1 : Vec<T>::N, U = 4;
+  __shared__ float red[4][64 * V];
   const int L = a.lanes, sub = threadIdx.x % L, line = threadIdx.x / L, lines = 256 / L;
   const int group = blockIdx.x % a.groups;
   const int64_t rb = blockIdx.x / a.groups;
-  const int col = (group * L + sub) * V, n = a.N - col;
+  const int col = (group * L + sub) * V, n = a.N - col, back = !SINGLE && n > 0 && n < V ? V - n : 0;
+  const int at = n > 0 ? col - back : 0;   // where a lane reads: the last piece further in front, and shifted
   const int64_t r1 = min(a.M, (rb + 1) * a.rows_per);
+  const bool ragged = !SINGLE && (group + 1) * L * V > a.N;
+  auto load = [&](const void* p, int64_t ld, int64_t row, Vec<T>& v) {
+    if constexpr (SINGLE) v.v[0] = ((const T*)p)[row * ld + at];
+    else v = load_vec((const T*)p + row * ld + at);
+  };
   float s[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) s[i] = 0.0f;
-  int64_t r = rb * a.rows_per + line;
-  if ((group + 1) * L * V <= a.N) {   // whole pieces: four rows under way
-    for (; r + 3 * lines < r1; r += 4 * lines) {
-      Vec<T> g[4], z[4];
+  for (int64_t r = rb * a.rows_per + line; r < r1; r += U * lines) {
+    Vec<T> g[U], z[U];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        g[u] = load_vec((const T*)a.dy + (r + u * lines) * a.lddy + col);
-        if (a.act != DISN_ACT_NONE) z[u] = load_vec((const T*)a.pre + (r + u * lines) * a.ldp + col);
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        float v[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = (float)g[u].v[i] * (a.act != DISN_ACT_NONE ? slope((float)z[u].v[i], a.act) : 1.0f);
-        if (a.dz) {
-          Vec<T> o;
-          narrow<T, V>(v, o.v);
-          store_vec((T*)a.dz + (r + u * lines) * a.ldz + col, o, V);
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) s[i] += v[i];
-      }
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = min(r + u * lines, r1 - 1);
+      load(a.dy, a.lddy, row, g[u]);
+      if (a.act != DISN_ACT_NONE) load(a.pre, a.ldp, row, z[u]);
     }
-  }
-  if (n > 0) {
-    for (; r < r1; r += lines) {
-      const Vec<T> g = load_vec((const T*)a.dy + r * a.lddy + col, n, col);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = r + u * lines;
+      if (row >= r1) break;
+      if (ragged) {
+        g[u] = shift_vec(g[u], back);
+        if (a.act != DISN_ACT_NONE) z[u] = shift_vec(z[u], back);
+      }
       float v[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = (float)g.v[i];
-      if (a.act != DISN_ACT_NONE) {
-        const Vec<T> z = load_vec((const T*)a.pre + r * a.ldp + col, n, col);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] *= slope((float)z.v[i], a.act);
-      }
-      if (a.dz) {
-        Vec<T> o;
-        narrow<T, V>(v, o.v);
-        store_vec((T*)a.dz + r * a.ldz + col, o, n);
+      for (int i = 0; i < V; ++i) v[i] = (float)g[u].v[i] * (a.act != DISN_ACT_NONE ? slope((float)z[u].v[i], a.act) : 1.0f);
+      if (a.dz && n > 0) {
+        T* dz = (T*)a.dz + row * a.ldz + col;
+        if constexpr (SINGLE) {
+          *dz = (T)v[0];
+        } else {
+          Vec<T> o;
+          narrow<T, V>(v, o.v);
+          store_vec(dz, o, n);
+        }
       }
 #pragma unroll
       for (int i = 0; i < V; ++i) s[i] += v[i];
     }
   }
   if (!a.part) return;
+  // a wave's rows by lane exchange, the four waves through LDS
 #pragma unroll
-  for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = s[i];
+  for (int i = 0; i < V; ++i) {
+    for (int d = L; d < 64; d <<= 1) s[i] += __shfl_xor(s[i], d, 64);
+    if ((threadIdx.x & 63) < L) red[threadIdx.x >> 6][sub * V + i] = s[i];
+  }
   __syncthreads();
   for (int t = threadIdx.x; t < L * V; t += 256) {
-    float z = red[t];
-    for (int l = 1; l < lines; ++l) z += red[l * L * V + t];
     const int j = group * L * V + t;
-    if (j < a.N) a.part[(size_t)rb * a.N + j] = z;
+    if (j < a.N) a.part[(size_t)rb * a.N + j] = (red[0][t] + red[1][t]) + (red[2][t] + red[3][t]);
   }
 }
 
 // ---- host: which kernel, which tile ------------------------------------------------------------------------------------
-enum Kind { K_EMPTY, K_SMALL, K_ROWS, K_TILE };
+enum Kind { K_EMPTY, K_SMALL, K_ROWS, K_OUTER, K_THIN, K_TILE };
 struct Product {
   const void *A, *B;
   int64_t lda, ldb;
@@ -1319,7 +1441,10 @@ double small_us(int type, const Product& q, bool gated = false) {
   const double K = (double)q.K, values = (double)mt * nt * 32 * K;
   const double chain = f32 ? 0.0027 * K : q.a_across || q.b_across ? 2.5e-6 * K * K : 0.0023 * K;
   const double rate = (f32 ? ((double)q.N * K > 8e6 ? 1.5e6 : 2.2e6) : 2e6) * (gated ? 0.4 : 1.0);
-  return 2.5 + (chain > values / rate ? chain : values / rate);
+  double us = chain > values / rate ? chain : values / rate;
+  const double stores = (double)q.M * q.N / 0.8e6;   // single values
+  if (us < stores) us = stores;
+  return 2.5 + us;
 }
 // The same of k_rows_*, up to four rows: W at 6.5 TB/s, and the sum of the parts as a launch more where W lies across r.
 // 4096 x 4096 in bf16 / fp32: one row 13.5 / 15.3 us across, 8.8 / 12.6 along r (k_small 43 / 22, 12 / 16; tiles 14 / 32),
@@ -1333,6 +1458,25 @@ double rows_us(int type, const Product& q) {
   return q.M > 1 ? 5.5 + 1.4 * us : 3.2 + us;
 }
 
+// lanes that share a row of n values, and groups of them along it
+int lanes_of(int64_t n, int V) {
+  int l = 1;
+  while (l < 64 && l * V < n) l *= 2;
+  return l;
+}
+// k_outer writes 4.5 TB/s; the loads of a row's values bound two and three products in 16 bits, and tiles are faster for more
+double outer_us(int type, const Product& q) {
+  const double results = (double)q.M * q.N;
+  if (type == DISN_F32) return q.K <= THIN ? 5 + results / 1.1e6 : 1e30;
+  return q.K == 1 ? 5 + results / 2.2e6 : q.K <= 3 ? 5 + results / 1e6 : 1e30;
+}
+// k_thin and the sum of its parts: the latter's launch, the loads of a row's values of the narrow operand, the wide one
+double thin_us(int type, const Product& q) {
+  const int64_t S = q.M < q.N ? q.M : q.N, D = q.M < q.N ? q.N : q.M;
+  if (type != DISN_F32 || !q.a_across || !q.b_across || S > THIN || D < 4) return 1e30;
+  return 13 + 0.8 * S + (double)q.K * (q.M + q.N) / 1.25e6;
+}
+
 Plan plan(int type, const Product& q) {
   Plan p{};
   const bool a_across = q.a_across, b_across = q.b_across;
@@ -1343,8 +1487,23 @@ Plan plan(int type, const Product& q) {
   const TileChoice c = choose_tile(type == DISN_F32, M, N, K, !pack_a && !pack_b);
   // (a copy of an operand takes 4 us and moves it twice)
   const double tile = c.us + (pack_a ? 4 + 4e-6 * M * K / 4 : 0) + (pack_b ? 4 + 4e-6 * N * K / 4 : 0);
-  const double rows = rows_us(type, q), small = small_us(type, q);
+  const double rows = rows_us(type, q), small = small_us(type, q), outer = outer_us(type, q), thin = thin_us(type, q);
   p.us = rows < small ? rows : small;
+  if (outer < p.us && outer < tile) {
+    p.kind = K_OUTER, p.us = outer;
+    return p;
+  }
+  if (thin < p.us && thin < tile) {
+    p.kind = K_THIN, p.us = thin;
+    const int64_t D = M < N ? N : M;
+    const int lanes = lanes_of(D, V);
+    const int64_t groups = ceil_div(D, lanes * V), least = 256 / lanes * 8;   // a step of a workgroup
+    p.per = ceil_div(K, ceil_div(512, groups));
+    p.per = ceil_div(p.per < least ? least : p.per, least) * least;
+    p.splits = (int)ceil_div(K, p.per);
+    p.bytes = (size_t)p.splits * M * N * sizeof(float);
+    return p;
+  }
   if (p.us < tile) {
     p.kind = rows < small ? K_ROWS : K_SMALL;
     if (p.kind == K_SMALL || !b_across) return p;
@@ -1451,6 +1610,32 @@ void launch_rows(const RowsArgs& a, bool b_across, int splits, hipStream_t strea
     k_rows_along<T, MR, 4><<<(unsigned)ceil_div(a.N, 4), 256, 0, stream>>>(a);
 }
 
+template <typename T>
+void launch_outer(const Product& q, hipStream_t stream) {
+  OuterArgs a{q.A, q.B, q.a_across ? 1 : q.lda, q.a_across ? q.lda : 1, q.b_across ? 1 : q.ldb, q.b_across ? q.ldb : 1, q.M, 0, (int)q.N, (int)q.K,
+              lanes_of(q.N, Vec<T>::N), 0, q.e};
+  a.groups = (int)ceil_div(q.N, a.lanes * Vec<T>::N);
+  const int64_t step = 256 / a.lanes * 4, most = ceil_div(2048, a.groups);
+  a.rows_per = ceil_div(ceil_div(q.M, most), step) * step;
+  const unsigned blocks = (unsigned)(ceil_div(q.M, a.rows_per) * a.groups);
+  if (q.K == 1) k_outer<T, 1><<<blocks, 256, 0, stream>>>(a);
+  else if (q.K <= 4) k_outer<T, 4><<<blocks, 256, 0, stream>>>(a);
+  if constexpr (sizeof(T) == 4)
+    if (q.K > 4) k_outer<T, THIN><<<blocks, 256, 0, stream>>>(a);
+}
+void launch_thin(const Product& q, const Plan& p, float* part, hipStream_t stream) {
+  const bool a_wide = q.M > q.N;
+  ThinArgs a{(const float*)(a_wide ? q.A : q.B), (const float*)(a_wide ? q.B : q.A), a_wide ? q.lda : q.ldb, a_wide ? q.ldb : q.lda, q.K, p.per, (int)(a_wide ? q.M : q.N),
+             (int)(a_wide ? q.N : q.M), 0, 0, a_wide ? q.N : 1, a_wide ? 1 : q.N, q.M * q.N, part};
+  a.lanes = lanes_of(a.D, 4);
+  a.groups = (int)ceil_div(a.D, a.lanes * 4);
+  const unsigned blocks = (unsigned)(a.groups * p.splits);
+  if (a.S == 1) k_thin<1><<<blocks, 256, 0, stream>>>(a);
+  else if (a.S == 2) k_thin<2><<<blocks, 256, 0, stream>>>(a);
+  else if (a.S <= 4) k_thin<4><<<blocks, 256, 0, stream>>>(a);
+  else k_thin<THIN><<<blocks, 256, 0, stream>>>(a);
+}
+
 SmallArgs small_args(const Product& q, const Plan&) {
   SmallArgs s{};
   s.A = {q.A, nullptr, q.lda, 0}, s.B = {q.B, nullptr, q.ldb, 0};
@@ -1499,6 +1684,16 @@ int run_product(DisnCtx* ctx, Product q, Plan p, char* ws, hipStream_t stream) {
     }
     DISN_HIP(ctx, hipGetLastError());
     return DISN_OK;
+  }
+  if (p.kind == K_OUTER) {
+    launch_outer<T>(q, stream);
+    DISN_HIP(ctx, hipGetLastError());
+    return DISN_OK;
+  }
+  if (p.kind == K_THIN) {
+    launch_thin(q, p, part, stream);
+    DISN_HIP(ctx, hipGetLastError());
+    return launch_finish<T>(ctx, part, p.splits, q.M, q.N, q.e, stream);
   }
   if (p.kind == K_ROWS) {
     RowsArgs r{q.A, q.B, q.lda, q.ldb, (int)q.M, (int)q.N, (int)q.K, (int)p.per, (int)ceil_div(q.N, 64 * Vec<T>::N), part, q.e};
@@ -1599,9 +1794,8 @@ GradPlan plan_backward(const DisnLinearGrad* a) {
   const double apart = products + 8 + 3e-6 * a->m * a->n * s / 5;
   g.small = a->m && a->n && a->k && a->dw && (a->dx ? small_us(a->type, dx, gated) : 0) + small_us(a->type, dw, gated) <= apart;
   if (g.small) return g;
-  const int V = (int)(16 / s);
-  g.gate_lanes = 1;
-  while (g.gate_lanes < 64 && g.gate_lanes * V < a->n) g.gate_lanes *= 2;
+  const int V = a->n < (int64_t)(16 / s) ? 1 : (int)(16 / s);
+  g.gate_lanes = lanes_of(a->n, V);
   g.gate_groups = (int)ceil_div(a->n, g.gate_lanes * V);
   if (g.gate_groups < 1) g.gate_groups = 1;
   // row blocks: about 1024 workgroups, at least 4 rows a thread
@@ -1631,7 +1825,9 @@ int run_backward(DisnCtx* ctx, const DisnLinearGrad* a, const GradPlan& g, char*
     if (a->n && a->m && (write || a->db)) {
       GateArgs k{a->dy, a->pre, write ? ws : nullptr, a->db ? (float*)(ws + g.off_sums) : nullptr, a->lddy, a->ldp, g.ldz, a->m,
                  g.gate_rows, (int)a->n, g.gate_lanes, g.gate_groups, a->act};
-      k_gate<T><<<(unsigned)(g.gate_groups * g.gate_blocks), 256, 0, stream>>>(k);
+      const unsigned blocks = (unsigned)(g.gate_groups * g.gate_blocks);
+      if (a->n < Vec<T>::N) k_gate<T, true><<<blocks, 256, 0, stream>>>(k);
+      else k_gate<T, false><<<blocks, 256, 0, stream>>>(k);
       DISN_HIP(ctx, hipGetLastError());
     }
     if (a->db && a->n) {

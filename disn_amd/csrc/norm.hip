@@ -250,25 +250,24 @@ __global__ __launch_bounds__(G <= 64 ? 256 : G) void k_layer_norm_backward(NormA
     }
   }
   if (!a.dweight && !a.dbias) return;
-  // the workgroup's sums: groups of one workgroup through LDS in group order, then out (one workgroup) or partial sums
-  constexpr int K = B / G;
-  __shared__ float red[K > 1 ? B * E : 1];
+  // the workgroup's sums: the groups of a wave by lane exchange, four waves through LDS, then out (one workgroup) or partial sums
+  constexpr int WAVES = G <= 64 ? 4 : 1;
+  __shared__ float red[WAVES > 1 ? WAVES * G * E : 1];
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     float(&v)[E] = which ? db : dg;
-    if constexpr (K > 1) {
+    if constexpr (WAVES > 1) {
       if (which) __syncthreads();
 #pragma unroll
-      for (int i = 0; i < E; ++i) red[threadIdx.x * E + i] = v[i];
+      for (int i = 0; i < E; ++i) {
+#pragma unroll
+        for (int m = G; m < 64; m <<= 1) v[i] += __shfl_xor(v[i], m, 64);
+        if ((threadIdx.x & 63) < G) red[((threadIdx.x >> 6) * G + t) * E + i] = v[i];
+      }
       __syncthreads();
       if (threadIdx.x < G) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          float s = red[threadIdx.x * E + i];
-#pragma unroll 2   // (all of them ahead are more registers than the rows need)
-          for (int k = 1; k < K; ++k) s += red[(k * G + threadIdx.x) * E + i];
-          v[i] = s;
-        }
+        for (int i = 0; i < E; ++i) v[i] = (red[t * E + i] + red[(G + t) * E + i]) + (red[(2 * G + t) * E + i] + red[(3 * G + t) * E + i]);
       }
     }
     if (threadIdx.x < G) {
