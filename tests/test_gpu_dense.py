@@ -314,6 +314,51 @@ def test_linear_float32_small_among_others(ctx, m, k, n):
     assert (y[1::6] == 0).all()
 
 
+# layers with few inputs, few outputs or few rows: sums of up to 8 products, results of up to 8 columns, and one beyond either
+NARROW = [(40000, 3, 70), (20000, 1, 515), (20000, 515, 1), (9617, 12, 2), (30011, 130, 5), (30000, 6, 257), (70001, 2, 9), (8, 3000, 2000),
+          (2, 2100, 3001), (30000, 8, 8), (30000, 9, 300), (30000, 300, 9), (70000, 4, 4), (70000, 3, 1)]
+
+
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("m,k,n", NARROW)
+def test_narrow_layers(ctx, m, k, n, kind, layout):
+    test_linear_whole_numbers(ctx, m, k, n, kind, layout)
+    test_linear_backward_whole_numbers(ctx, m, k, n, kind, layout)
+
+
+@pytest.mark.parametrize("act", ["none", "gelu"])
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("m,k,n", NARROW)
+def test_narrow_layers_values(ctx, m, k, n, kind, act):
+    test_linear_values(ctx, m, k, n, kind, act)
+    test_linear_backward_values(ctx, m, k, n, kind, act)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("m,k,n", [(40000, 3, 70), (20000, 515, 1), (9617, 12, 2), (30000, 6, 257), (2, 2100, 3001)])
+def test_narrow_layers_rows_anywhere(ctx, m, k, n, kind):
+    test_linear_rows_anywhere(ctx, m, k, n, kind)
+    g = gen(m, k, n, kind, 10)
+    x, w, r = (ints(g, kind, *s) for s in ((m, k), (k, n), (m, n)))
+    want = x.double() @ w.double() + r.double()
+    assert ctx.linear(x, w, residual=r, out=r) is r        # in place
+    same(r, want)
+
+
+@pytest.mark.parametrize("m,k,n", [(40000, 3, 70), (30000, 515, 2)])
+def test_narrow_layers_infinities_and_nan(ctx, m, k, n):
+    g = gen(m, k, n, 11)
+    x, w, dy = ints(g, "f32", m, k), ints(g, "f32", k, n), ints(g, "f32", m, n)
+    x[7, 1], dy[9, 0] = float("nan"), float("inf")
+    y = ctx.linear(x, w)
+    assert torch.equal(y.isnan().any(1).nonzero().flatten(), torch.tensor([7], device=DEV))
+    dx, dw, db = ctx.linear_backward(dy, x, w)
+    assert torch.equal((~dx.isfinite()).any(1).nonzero().flatten(), torch.tensor([9], device=DEV))
+    assert dw[1].isnan().all() and not dw[0, 1:].isnan().any() and not dw[2:, 1:].isnan().any()
+    assert db[0] == float("inf") and db[1:].isfinite().all()
+
+
 def norm_inputs(rows, d, kind, seed):
     g = gen(rows, d, kind, seed)
     x = (torch.randn(rows, d, generator=g, device=DEV) * (0.2 + 3 * torch.rand(rows, 1, generator=g, device=DEV)) +
