@@ -323,7 +323,7 @@ __device__ __forceinline__ TilePlace tile_place(const TileArgs& a, int block, in
 // FMA's rounding is.  Six bf16 MFMAs take 6/16 of the time of one fp32 MFMA of the same size.  Infinities,
 // NaN and intermediate overflow cannot be cut; a tile whose sums are not all finite is computed again by fp32 MFMAs.
 // Neither can values below 2^-109, whose last term's bits lie below bf16's smallest; a tile that met one (an or over the
-// last terms: an instruction for two values, 2 % of the time) looks whether its sums are small enough to notice, and is computed again if so.
+// last terms: an instruction for two values, under 1 % of the time) looks whether its sums are small enough to notice, and is computed again if so.
 //
 // LDS: an operand along r as [8 r][i][16 bytes] (half a fragment is 512 bytes in one piece; 128 bytes between the 8-r
 // blocks put the lanes that store a row on different banks); an operand across r as [r][i] with 64 bytes between rows,
@@ -411,11 +411,12 @@ struct Operand {
       }
 #pragma unroll
       for (int p = 0; p < P; ++p) {
-        bf16_t term[4];
-        narrow<bf16_t, 4>(rest, term);
+        // (a bf16 is the upper half of a float; widened as values, hipcc converts every value a second time)
+        uint32_t term[2];
+        narrow<bf16_t, 4>(rest, (bf16_t*)term);
         if (p + 1 < P) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) rest[i] -= (float)term[i];
+          for (int i = 0; i < 4; ++i) rest[i] -= __builtin_bit_cast(float, i & 1 ? term[i / 2] & 0xffff0000u : term[i / 2] << 16);
         }
         __builtin_memcpy(__builtin_assume_aligned(dst + p * PLANE, 8), term, 8);
         if (p + 2 == P) {
@@ -604,13 +605,12 @@ __device__ __forceinline__ void tile32(const TileArgs& a, int block, char* lds) 
       fetch(slot, s + 1 + DEPTH);
     }
     if (WHOLE) {
-      // the cutting of stage s + 1 runs between the matrix instructions of stage s, so many of its instructions behind each
-      // (100000 x 1984 x 512, W across: 6 984 us, 4 969; along: 6 947, 5 926, 4 946; 16384 x 512 x 512 in 128-wide tiles: 6 55.5, 4 57)
-      constexpr int BETWEEN = BM == 128 ? 6 : B_ACROSS ? 4 : 5;
+      // the cutting of stage s + 1 runs between the matrix instructions of stage s, up to four of its instructions behind each
+      // (16384 x 512 x 512: 53.7 us, one 54.6, six 55)
 #pragma unroll
       for (int i = 0; i < MB * NB * 6; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x2, BETWEEN, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
       }
     }
   };
