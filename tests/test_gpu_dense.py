@@ -523,6 +523,30 @@ def test_residual_block(ctx, points, d, wide, kind):
         assert (a.double() - b).norm() <= tol * b.norm()
 
 
+def test_inside_an_autograd_function(ctx):
+    """the two halves of a layer behind torch's own gradients; y serves as the backward pass's z"""
+    class Dense(torch.autograd.Function):
+        @staticmethod
+        def forward(c, x, w, b):
+            y = ctx.linear(x, w, b, act="relu")
+            c.save_for_backward(x, w, y)
+            return y
+
+        @staticmethod
+        def backward(c, dy):
+            x, w, y = c.saved_tensors
+            return ctx.linear_backward(dy, x, w, pre=y, act="relu")
+
+    g = gen(12)
+    x, w, b = (ints(g, "f32", *s).requires_grad_() for s in ((2, 50, 70), (70, 33), (33,)))
+    Dense.apply(x, w, b).sum().backward()                  # the gradient of a sum arrives as one value, expanded
+    got = [t.grad for t in (x, w, b)]
+    leaves = [t.detach().double().requires_grad_() for t in (x, w, b)]
+    torch.relu(leaves[0] @ leaves[1] + leaves[2]).sum().backward()
+    for a, want in zip(got, leaves):
+        same(a, want.grad)
+
+
 def test_same_bits_every_time(ctx):
     for kind in KINDS:
         x, p, dy = block_inputs(3000, 256, 300, kind, 1)
