@@ -14,8 +14,9 @@
 // row while it works on the present one (us without / with, 300 MB of bf16 rows: d = 768 343 / 167, 1024 276 / 168,
 // 4096 300 / 189); so does the forward pass of the longest rows (d = 5000 168 / 127).
 // Measured: 262144 x 512 bf16 forward 106 us (5.1 TB/s of what is read and written), backward with a residual 194 us (5.5), 5003 x 1537
-// fp32 backward 25 us (3.7).  Rows of 16-bit values that start at odd places are slower, 16 bytes of them at a time cost the
-// memory pipe two accesses: 300 MB in rows of 1031 forward 198 us, backward 325; of 1024 114 and 176.
+// fp32 backward 25 us (3.7).  Rows of 16-bit values that start at odd places are slower:
+// 300 MB in rows of 1031 forward 198 us, backward 325; of 1024 114 and 176 (read as aligned dwords and shifted 182 and 357,
+// stored in three aligned pieces 213 and 336).
 #include "dense.h"
 
 namespace {
