@@ -120,7 +120,7 @@ __device__ __forceinline__ void finish_vec(const Epilogue& e, T* out, T* pre, fl
   Vec<T> o;
   if (e.pre) {
     narrow<T, N>(z, o.v);
-    store_vec(pre, o, n);
+    store_vec<T, true>(pre, o, n);
   }
   activate_all(z, e.act);
   if (e.residual) {
@@ -128,7 +128,7 @@ __device__ __forceinline__ void finish_vec(const Epilogue& e, T* out, T* pre, fl
     for (int i = 0; i < N; ++i) z[i] += (float)residual.v[i];
   }
   narrow<T, N>(z, o.v);
-  store_vec(out, o, n);
+  store_vec<T, true>(out, o, n);
 }
 template <typename T>
 __device__ __forceinline__ Vec<T> bias_vec(const Epilogue& e, int col, int n) {
@@ -274,7 +274,7 @@ __device__ __forceinline__ void tile_end(const TileArgs& a, int split, int iw, i
         }
         Vec<T> o;
         narrow<T, V>(z, o.v);
-        __builtin_memcpy(out, &o, 16);
+        stream_vec(out, o);
         out += out_step;
       }
       continue;

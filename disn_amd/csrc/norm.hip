@@ -173,7 +173,7 @@ __global__ __launch_bounds__(G <= 64 ? 256 : G) void k_layer_norm(NormArgs a) {
 #pragma unroll
       for (int i = 0; i < N; ++i) x[p * N + i] = fmaf(x[p * N + i] * rstd, w[p * N + i], b[p * N + i]);
       narrow<T, N>(x + p * N, o.v);
-      store_vec(y + c, o, ENDS == WHOLE ? N : d - c);
+      store_vec<T, true>(y + c, o, ENDS == WHOLE ? N : d - c);
     }
   }
 }
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(G <= 64 ? 256 : G) void k_layer_norm_backward(NormA
         g[e] = v;
       }
       narrow<T, N>(g + p * N, o.v);
-      store_vec(dx + c, o, ENDS == WHOLE ? N : d - c);
+      store_vec<T, true>(dx + c, o, ENDS == WHOLE ? N : d - c);
     }
   }
   if (!a.dweight && !a.dbias) return;
