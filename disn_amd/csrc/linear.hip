@@ -668,8 +668,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile32(TileArgs a) {
 // instructions), so all but one of its stages are on their way while one is multiplied.  Two steps of 16 r a stage, and
 // the fragments of a step are read while the step before is multiplied; the one barrier of a stage lies between its two
 // steps, when the second step's fragments are in registers: no wave waits for LDS behind it.  Bound by the matrix cores, then
-// by the epilogue, which no other workgroup of the CU covers: 65536 x 1536 x 512 bf16 96 us (1.07 PFLOP/s), its weight's
-// gradient 94 and the input's, with three times the results, 130; 4096^3 113 to 125 (a library product 104 to 125).
+// by the epilogue, which no other workgroup of the CU covers: 65536 x 1536 x 512 bf16 91 us (1.13 PFLOP/s), its weight's
+// gradient 88 and the input's, with three times the results, 117; 4096^3 113 to 125 (a library product 104 to 125).
 //
 // A wave's DMA writes 1 KB of LDS in lane order, from any 16-byte pieces of memory.  Along r, LDS holds [i][32 r] (64
 // bytes), and the four pieces of a row are exchanged by (i >> 2) & 3: sixteen lanes of a fragment, sixteen rows, touch
@@ -1152,7 +1152,7 @@ __global__ __launch_bounds__(256) void k_rows_along(RowsArgs a) {
 // ---- k_outer: sums of up to 8 products ---------------------------------------------------------------------------------
 // (the first layer of three coordinates; gradients of a layer with few outputs or of few rows).  Bound by writing C: a lane
 // keeps its 16 bytes of columns of B and walks over rows, several of them under way.
-// 262144 x 512 results of one product: bf16 49 us (5.5 TB/s), k_small 152; fp32 135 and 186; of three products in fp32, 65536
+// 262144 x 512 results of one product: bf16 54 us (5.0 TB/s), k_small 152; fp32 109 and 186; of three products in fp32, 65536
 // rows 36 and 45.  In 16 bits more products are faster in tiles (65536 x 512 of three 24 us, here 37; but 262144 x 64 here 25,
 // k_small 35).
 struct OuterArgs {
