@@ -88,7 +88,9 @@ template <typename T>
 __device__ __forceinline__ void stream_vec(T* p, const Vec<T>& r) {
   typedef __attribute__((ext_vector_type(4))) uint32_t four;
   typedef four words __attribute__((aligned(2)));   // any address that fits T
+  asm volatile("");   // (without the two, a branch between this store and an ordinary one becomes one ordinary store)
   __builtin_nontemporal_store(__builtin_bit_cast(words, r), (words*)p);
+  asm volatile("");
 }
 // the first n (n >= N: all) values to p
 template <typename T, bool STREAM = false>
