@@ -13,6 +13,8 @@
 //   k_outer  sums of up to 8 products: C is what takes time to write
 //   k_thin   long sums for a C of up to 8 rows or columns: the wider operand is what takes time to read
 #include "dense.h"
+#define EDGE_QUAL __device__ __forceinline__
+#include "tile_edge.h"
 
 #include <atomic>
 #include <type_traits>
@@ -357,7 +359,7 @@ struct Operand {
   int left;          // i values in the tile
   int first;         // the stage's first value in its row
   int lines;         // i values in the matrix
-  int back[ACROSS ? Q : 1];   // how far in front a piece that holds the last column is read
+  int back[ACROSS ? Q : 1];   // how far in front a piece is read in whole stages (inside() lines)
   Vec<T> reg[DEPTH][Q];   // stages under way
 
   __device__ __forceinline__ void init(const T* p, int64_t ld_, int i0, int n_i, int64_t k0) {
@@ -368,12 +370,14 @@ struct Operand {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int t = threadIdx.x + q * THREADS, line = t / PER_LINE, c = t % PER_LINE * V;
-      if (ACROSS) back[q] = c < left && left < c + V ? c + V - left : 0;
-      // places outside the matrix read its nearest line or first piece instead: they only reach sums nobody stores
-      if (ACROSS)
-        ptr[q] = p + (k0 + line) * ld + i0 + (c < left ? c : 0);
-      else
+      // places outside the matrix read its nearest line or the tile's first piece instead: they only reach sums nobody stores
+      if (ACROSS) {
+        const EdgePiece e = edge_piece(c, left, V);
+        back[q] = e.back;
+        ptr[q] = p + (k0 + line) * ld + i0 + e.at;
+      } else {
         ptr[q] = p + (int64_t)(i0 + (line < left ? line : left - 1)) * ld + k0 + c;
+      }
     }
   }
   // whether whole stages need no ends to be cut
