@@ -450,9 +450,10 @@ struct Operand {
   }
 };
 
-// The largest absolute value of n (<= WIDTH) lines' r values k0 .. k0 + have - 1, for every thread; lds: a float a wave
+// Over n (<= WIDTH) lines' r values k0 .. k0 + have - 1: the largest absolute value, for every thread, and 1 in live[] for every line
+// that holds anything but zeros (0 there before; complete behind the caller's next barrier).  lds: a float a wave
 template <bool ACROSS, int WIDTH, int THREADS>
-__device__ __forceinline__ float panel_max(const float* p, int64_t ld, int line, int n, int64_t k0, int have, float* lds) {
+__device__ __forceinline__ float panel_max(const float* p, int64_t ld, int line, int n, int64_t k0, int have, float* lds, uint8_t* live) {
   p += ACROSS ? k0 * ld + line : line * ld + k0;
   // 16 bytes a thread of a run of contiguous values; the last piece of a run lies over the one before it
   constexpr int PER = ACROSS ? WIDTH / 4 : 64;
@@ -460,12 +461,27 @@ __device__ __forceinline__ float panel_max(const float* p, int64_t ld, int line,
   float most = 0.0f;
   for (int c0 = 0; c0 < run; c0 += PER * 4) {
     const int c = c0 + (int)threadIdx.x % PER * 4, at = min(c, max(run - 4, 0));
+    float column[4] = {0, 0, 0, 0};   // (ACROSS) the largest of each of the four lines
 #pragma unroll 8
     for (int t = threadIdx.x / PER; t < runs; t += THREADS / PER) {
       Vec<float> v;
       if (run >= 4) v = load_vec(p + t * ld + at);
       else v = load_vec(p + t * ld, run, 0);
-      most = fmaxf(fmaxf(most, fmaxf(fabsf(v.v[0]), fabsf(v.v[1]))), fmaxf(fabsf(v.v[2]), fabsf(v.v[3])));
+      if (ACROSS) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) column[i] = fmaxf(column[i], fabsf(v.v[i]));
+      } else {
+        const float here = fmaxf(fmaxf(fabsf(v.v[0]), fabsf(v.v[1])), fmaxf(fabsf(v.v[2]), fabsf(v.v[3])));
+        if (here > 0.0f) live[t] = 1;
+        most = fmaxf(most, here);
+      }
+    }
+    if (ACROSS) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (column[i] > 0.0f) live[at + i] = 1;
+        most = fmaxf(most, column[i]);
+      }
     }
   }
 #pragma unroll
@@ -646,17 +662,29 @@ __device__ __forceinline__ void tile32(const TileArgs& a, int block, char* lds) 
         for (int g = 0; g < 16; ++g) bad |= !(fabsf(acc[m][n][g]) <= 3.4028235e38f);
     bool again = __syncthreads_or(bad || (lost & 0xffff));
     if (again && !__syncthreads_or(bad)) {
-      // Bits were lost, at most 2^-134 of a value.  Does a sum notice, is it below 2^24 times what all of its products may
-      // have lost?  A sum of 0 (an empty row) is left at 0 where that is below 2^-100.
-      const float most = panel_max<A_ACROSS, BM, THREADS>((const float*)a.A, a.lda, i0, min(a.M - i0, BM), k0, have, (float*)lds) +
-                         panel_max<B_ACROSS, BN, THREADS>((const float*)a.B, a.ldb, j0, min(a.N - j0, BN), k0, have, (float*)lds);
-      const float least = most * (float)have * 0x1p-109f;
+      // Bits were lost, at most 2^-134 of a value.  Does a sum notice: can all of its products together have lost enough to reach
+      // the result's smallest step, and is it below 2^25 times that?  A sum of 0 is one where its row of A or its column of B holds
+      // nothing else; lines outside the matrix count as such.
+      uint8_t *live_a = (uint8_t*)lds + 64, *live_b = live_a + BM;
+      for (int t = threadIdx.x; t < BM + BN; t += THREADS) live_a[t] = 0;
+      __syncthreads();
+      const float reach = (float)have * (panel_max<A_ACROSS, BM, THREADS>((const float*)a.A, a.lda, i0, min(a.M - i0, BM), k0, have, (float*)lds, live_a) +
+                                         panel_max<B_ACROSS, BN, THREADS>((const float*)a.B, a.ldb, j0, min(a.N - j0, BN), k0, have, (float*)lds, live_b));
+      if (reach > 0x1p-26f) {   // each part of a split sum (1024 at most) may lose 2^-160, half a step of 2^-149 in all
+        const float least = reach * 0x1p-109f;
+        const int lane = threadIdx.x & 63;
+        bool column[NB];
 #pragma unroll
-      for (int m = 0; m < MB; ++m)
+        for (int n = 0; n < NB; ++n) column[n] = live_b[wj + n * 32 + (lane & 31)];
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+        for (int m = 0; m < MB; ++m)
 #pragma unroll
-          for (int g = 0; g < 16; ++g) bad |= fabsf(acc[m][n][g]) < least && (acc[m][n][g] != 0.0f || least > 0x1p-76f);
+          for (int g = 0; g < 16; ++g) {
+            const bool row = live_a[wi + m * 32 + 4 * (lane >> 5) + (g & 3) + 8 * (g >> 2)];
+#pragma unroll
+            for (int n = 0; n < NB; ++n) bad |= fabsf(acc[m][n][g]) < least && (acc[m][n][g] != 0.0f || (row && column[n]));
+          }
+      }
       again = __syncthreads_or(bad);
     }
     if (again) fp32_sums<A_ACROSS, B_ACROSS, MB, NB>(a, i0 + wi, j0 + wj, k0, have, acc);

@@ -69,3 +69,39 @@ def test_contents_of_the_workspace(ctx, m, k, n, kind, w_nk):
         first = first or (dx, dw, db)
         assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), first)), what
     assert all(v.isfinite().all() for v in first)
+
+
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("xs,ws", [(-140, 20), (-140, 30), (-138, 8), (-136, 0), (30, -141), (-149, 12), (-107, 3), (-104, 80), (-111, 60)])
+@pytest.mark.parametrize("m,k,n", [(300, 700, 800), (3000, 900, 1100), (3000, 512, 1100), (40000, 200, 260)])
+def test_float32_values_below_the_terms(ctx, m, k, n, xs, ws, layout):
+    """values that the first or the last of three narrower terms cannot hold, with others that lift their products into the range"""
+    g = gen(m, k, n, xs, ws, "terms")
+    x = (torch.randn(m, k, generator=g, device=DEV).double() * 2.0 ** xs).float()
+    w = (torch.randn(k, n, generator=g, device=DEV).double() * 2.0 ** ws).float()
+    # (k + 4) roundings as everywhere, and six partial sums that may each be rounded to steps of 2^-149 a term
+    bound = 2 * (k + 4) * E * (x.double().abs() @ w.double().abs()) + 6 * (k + 4) * 2.0 ** -149
+    within(ctx.linear(x, weight(w, layout)), x.double() @ w.double(), bound)
+    dy = x.repeat(1, n // k + 1)[:, :n].contiguous()
+    dx, _, _ = ctx.linear_backward(dy, x, weight(w, layout))
+    within(dx, dy.double() @ w.double().t(), 2 * (n + 4) * E * (dy.double().abs() @ w.double().abs().t()) + 6 * (n + 4) * 2.0 ** -149)
+
+
+@pytest.mark.parametrize("m,k,n", [(300, 700, 803), (3000, 900, 1101), (40000, 200, 259)])
+def test_float32_smallest_values_between_zeros(ctx, m, k, n):
+    """rows and columns of nothing but zeros, next to rows that hold one value below the smallest of a narrower type"""
+    g = gen(m, k, n, "one")
+    x, w = torch.zeros(m, k, device=DEV), torch.randn(k, n, generator=g, device=DEV)
+    at = torch.randint(0, k, (m,), generator=g, device=DEV)
+    x[torch.arange(m, device=DEV), at] = 2.0 ** -140
+    x[::3] = torch.randn(x[::3].shape, generator=g, device=DEV)
+    x[1::6] = 0.0
+    w[:, ::7] = 0.0
+    w *= 2.0 ** 16
+    y, want = ctx.linear(x, w), x.double() @ w.double()
+    bound = 2 * (k + 4) * E * (x.double().abs() @ w.double().abs()) + 6 * (k + 4) * 2.0 ** -149
+    within(y, want, bound)
+    assert (y[1::6] == 0).all() and (y[:, ::7] == 0).all()
+    # one product a sum: exact
+    one = torch.arange(2, m, 6, device=DEV)
+    assert torch.equal(y[one], want[one].float())
