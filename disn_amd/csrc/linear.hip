@@ -77,20 +77,20 @@ __device__ __forceinline__ void activate_all(float (&z)[N], int act) {
       break;
   }
 }
-// act'(z)
-__device__ __forceinline__ float slope(float z, int act) {
+// dy act'(z)
+__device__ __forceinline__ float gated(float dy, float z, int act) {
   switch (act) {
-    case DISN_ACT_RELU: return z > 0.0f ? 1.0f : z <= 0.0f ? 0.0f : z;
+    case DISN_ACT_RELU: return z > 0.0f ? dy : z <= 0.0f ? 0.0f : z;   // a choice: closed, it passes nothing of an infinity either
     case DISN_ACT_GELU: {
       float e;
       const float q = normal_tail(fabsf(z), e);
-      return fmaf(z * 0.39894228f, e, z > 0.0f ? 1.0f - q : q);
+      return dy * fmaf(z * 0.39894228f, e, z > 0.0f ? 1.0f - q : q);
     }
     case DISN_ACT_SILU: {
       const float s = logistic(z);
-      return s * fmaf(z, 1.0f - s, 1.0f);
+      return dy * (s * fmaf(z, 1.0f - s, 1.0f));
     }
-    default: return 1.0f;
+    default: return dy;
   }
 }
 
@@ -975,7 +975,7 @@ __device__ __forceinline__ floatx4 small_operand(const SmallOperand& o, int i, i
     if (act != DISN_ACT_NONE) {
       const floatx4 z = load_4r<T, ACROSS, FULL>(o.gate, o.ldg, i, r0, K);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] *= FULL || r0 + e < K ? slope(z[e], act) : 1.0f;
+      for (int e = 0; e < 4; ++e) v[e] = FULL || r0 + e < K ? gated(v[e], z[e], act) : 0.0f;
     }
   }
   return v;
@@ -1352,7 +1352,7 @@ __global__ __launch_bounds__(256) void k_gate(GateArgs a) {
       }
       float v[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = (float)g[u].v[i] * (a.act != DISN_ACT_NONE ? slope((float)z[u].v[i], a.act) : 1.0f);
+      for (int i = 0; i < V; ++i) v[i] = a.act != DISN_ACT_NONE ? gated((float)g[u].v[i], (float)z[u].v[i], a.act) : (float)g[u].v[i];
       if (a.dz && n > 0) {
         T* dz = (T*)a.dz + row * a.ldz + col;
         if constexpr (SINGLE) {
@@ -1473,7 +1473,7 @@ Product rest_of(int type, Product q, int64_t cut) {
 // What k_small takes, in us; measured for 1 .. 256 rows and weights of 256^2 .. 4096^2.  Either one workgroup's chain of steps
 // along r bounds it (16-bit operands across r come in single values: 43 us at r = 4096, 6 at 1024), or the values that all
 // workgroups fetch: 2.2e6 a us in fp32 from L2, 1.5e6 from beyond it (weights of more than 32 MB), 2e6 in 16 bits.
-// Where an operand is gated, its slope is computed again in every workgroup that reads it: 0.4 of that rate (4099 rows
+// Where an operand is gated, its gate is computed again in every workgroup that reads it: 0.4 of that rate (4099 rows
 // of 515 x 257, fp32 silu: 201 us for both gradients; 62 in tiles).
 double small_us(int type, const Product& q, bool gated = false) {
   const int64_t mt = ceil_div(q.M, 16), nt = ceil_div(q.N, 16);

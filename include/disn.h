@@ -225,11 +225,12 @@ int disn_linear_workspace(DisnCtx* ctx, const DisnLinear* a, size_t* bytes);
 int disn_linear(DisnCtx* ctx, const DisnLinear* a, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Gradients of disn_linear: dz = dy act'(pre);  dx = dz W^T;  dw = x^T dz;  db = sum of dz over the rows.
+ * DISN_ACT_RELU: dz is dy where pre > 0 and 0 where pre <= 0, whatever dy is there (an infinity, a NaN).
  *   dy [m][n] (also the gradient of the residual);  pre [m][n]: z as disn_linear returned it, NULL with
  *   DISN_ACT_NONE; for DISN_ACT_RELU any tensor that is positive where z is does, y of a call without residual too
  *   dx [m][k], dw (layout w_nk, like w), db [n]: NULL = not wanted; w may be NULL without dx, x without dw
- * act'(0) of relu is 0; where pre is NaN, dz is NaN.  16-bit types: dz is rounded to the type before the two
- * products (they take 16-bit operands) unless act is none. */
+ * Where pre is NaN, dz is NaN.  16-bit types: dz is rounded to the type before the two products (they take 16-bit
+ * operands) unless act is none. */
 typedef struct DisnLinearGrad {
   int32_t type, act, w_nk, reserved; /* reserved = 0 */
   int64_t m, n, k;

@@ -105,3 +105,29 @@ def test_float32_smallest_values_between_zeros(ctx, m, k, n):
     # one product a sum: exact
     one = torch.arange(2, m, 6, device=DEV)
     assert torch.equal(y[one], want[one].float())
+
+
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("m,k,n", [(1, 5, 7), (20, 40, 30), (32, 1024, 512), (2, 2100, 3001), (3000, 900, 1100), (30000, 515, 2), (40000, 3, 70)])
+def test_infinite_gradients_at_a_closed_relu(ctx, m, k, n, kind, layout):
+    """what is not passed does not matter, be it an infinity or a NaN; a NaN in pre is still seen"""
+    g = gen(m, k, n, kind, layout, "closed")
+    x, w, dy, pre = (torch.randn(*s, generator=g, device=DEV).to(KINDS[kind]) for s in ((m, k), (k, n), (m, n), (m, n)))
+    w = weight(w, layout)
+    pre[0, 0], pre[m - 1, n - 1] = 0.0, -0.0
+    closed = pre <= 0
+    dy[closed] = 1.0
+    want = ctx.linear_backward(dy, x, w, pre=pre, act="relu")
+    for value in (float("inf"), float("-inf"), float("nan")):
+        dy[closed] = value
+        for a, b in zip(ctx.linear_backward(dy, x, w, pre=pre, act="relu"), want):
+            assert torch.equal(a, b), value
+        _, _, db = ctx.linear_backward(dy, None, None, pre=pre, act="relu", want_dx=False, want_dw=False)
+        assert db.isfinite().all()
+    dy[0, 0], pre[0, 0] = float("inf"), 1.0
+    dx, dw, db = ctx.linear_backward(dy, x, w, pre=pre, act="relu")
+    assert not dx[0].isfinite().any() and dx[1:].isfinite().all() and db[0] == float("inf") and db[1:].isfinite().all()
+    dy[0, 0], pre[0, 0] = 1.0, float("nan")
+    dx, dw, db = ctx.linear_backward(dy, x, w, pre=pre, act="relu")
+    assert dx[0].isnan().all() and dx[1:].isfinite().all() and db[0].isnan() and db[1:].isfinite().all()
