@@ -110,6 +110,41 @@ struct Row {
   }
 };
 
+// Whether all values of a row are equal: their mean is that value then, so that the row gives the bias (and 0 / 0 without an
+// eps).  A sum of equal fp32 values is rounded, and its mean may be some steps off; one of up to 8192 16-bit values is exact, so
+// there is nothing to do for those.  Waves that share a row leave their verdict in the upper half of the sum's slot.
+template <typename T, int G, int E>
+struct Equal {
+  float first;   // a value of the row
+  bool other;    // whether this group of lanes has met another
+  __device__ __forceinline__ Equal(const float (&x)[E], int t, int d, float* slot) {
+    if constexpr (sizeof(T) == 4) {
+      const int lane = threadIdx.x & 63, base = G < 64 ? lane & ~(G - 1) : 0;   // (every wave's first lane holds values of the row)
+      first = __shfl(x[0], base, 64);
+      bool o = false;
+#pragma unroll
+      for (int i = 0; i < E; ++i) o |= piece_col<T, G>(t, i / Vec<T>::N) + i % Vec<T>::N < d && x[i] != first;
+      const uint64_t met = __ballot(o) >> base;
+      other = (G < 64 ? met & ((1ull << (G & 63)) - 1) : met) != 0;
+      if (G > 64 && lane == 0) slot[8 + (threadIdx.x >> 6)] = other ? __builtin_nanf("") : first;
+    }
+  }
+  // behind the sum's barrier
+  __device__ __forceinline__ float mean_or(float mean, const float* slot) const {
+    if constexpr (sizeof(T) == 4) {
+      bool all = !other;
+      if constexpr (G > 64) {
+        all = true;
+#pragma unroll
+        for (int i = 0; i < G / 64; ++i) all &= slot[8 + i] == slot[8];   // (a NaN is not equal to itself)
+        return all ? slot[8] : mean;
+      }
+      return all ? first : mean;
+    }
+    return mean;
+  }
+};
+
 template <typename T, int G, int E, Ends ENDS>
 __global__ __launch_bounds__(G <= 64 ? 256 : G) void k_layer_norm(NormArgs a) {
   constexpr int N = Vec<T>::N, P = E / N, B = G <= 64 ? 256 : G;
@@ -149,7 +184,8 @@ __global__ __launch_bounds__(G <= 64 ? 256 : G) void k_layer_norm(NormArgs a) {
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < E; ++i) s += x[i];   // places behind the row hold 0
-    const float mean = group_sum<G>(s, lds, 0) / (float)d;   // a division: the mean of equal values is that value
+    const Equal<T, G, E> equal(x, t, d, lds[0]);
+    const float mean = equal.mean_or(group_sum<G>(s, lds, 0) / (float)d, lds[0]);
     s = 0.0f;
 #pragma unroll
     for (int p = 0; p < P; ++p)

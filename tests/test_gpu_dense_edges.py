@@ -131,3 +131,36 @@ def test_infinite_gradients_at_a_closed_relu(ctx, m, k, n, kind, layout):
     dy[0, 0], pre[0, 0] = 1.0, float("nan")
     dx, dw, db = ctx.linear_backward(dy, x, w, pre=pre, act="relu")
     assert dx[0].isnan().all() and dx[1:].isfinite().all() and db[0].isnan() and db[1:].isfinite().all()
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("d", [3, 40, 100, 200, 500, 1000, 1024, 1500, 2048, 3001, 5000, 8192])
+def test_rows_of_one_value(ctx, d, kind):
+    """the mean of equal values is that value, so the row gives the bias, and without an eps 0 / 0"""
+    values = torch.tensor([0.1, 0.7, -1.3, 1e-3, 12345.678, 1e30 if kind != "f16" else 3e4, 3e-39 if kind != "f16" else 3e-7, 0.0], device=DEV)
+    x = values.to(KINDS[kind])[:, None].expand(-1, d).contiguous()
+    g = gen(d, kind, "equal")
+    w, b = (torch.randn(d, generator=g, device=DEV).to(KINDS[kind]) for _ in range(2))
+    y, mean, rstd = ctx.layer_norm(x, w, b, eps=1e-5, want_stats=True)
+    assert torch.equal(mean, x[:, 0].float())
+    assert torch.equal(y, b.expand(len(values), d))
+    assert (rstd.double() - 1e-5 ** -0.5).abs().max() <= 4 * E * 1e-5 ** -0.5
+    assert ctx.layer_norm(x, w, b, eps=0.0).isnan().all()
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("d", [40, 200, 1000, 1500, 3001, 8192])
+def test_rows_far_from_zero(ctx, d, kind):
+    """a spread that is small beside the mean: the distances from the mean are as exact as the values allow"""
+    g = gen(d, kind, "far")
+    step = torch.finfo(KINDS[kind]).eps                      # of values from 1 to 2
+    x = (1.5 + step * torch.randint(-9, 10, (60, d), generator=g, device=DEV)).to(KINDS[kind])
+    eps = 1e-30
+    y, mean, rstd = ctx.layer_norm(x, eps=eps, want_stats=True)
+    mu = x.double().mean(1, keepdim=True)
+    c = x.double() - mu
+    r = (c * c).mean(1, keepdim=True) ** -0.5
+    within(mean, mu[:, 0], 2 * E * mu[:, 0])                 # a rounded value, corrected once and rounded again
+    # c is off by the mean's rounding, half a step of 2^-23 at most, in every value alike
+    err = 2 * 2 * E * r * (1 + (c * r).abs()) + 60 * E * (c * r).abs()
+    within(y, c * r, err + U[kind] * ((c * r).abs() + err) + 1e-7 * (kind == "f16"))
