@@ -164,3 +164,19 @@ def test_rows_far_from_zero(ctx, d, kind):
     # c is off by the mean's rounding, half a step of 2^-23 at most, in every value alike
     err = 2 * 2 * E * r * (1 + (c * r).abs()) + 60 * E * (c * r).abs()
     within(y, c * r, err + U[kind] * ((c * r).abs() + err) + 1e-7 * (kind == "f16"))
+
+
+def test_gelu_of_float32(ctx):
+    """gelu and its slope where most values lie, to the roundings of a few operations (one input, a weight of 1: z is x)"""
+    g = gen("gelu")
+    z = torch.rand(60000, 1, generator=g, device=DEV) * 2.4 - 1.2
+    one = torch.ones(1, 1, device=DEV)
+    wide = z.double()
+    cdf, density = 0.5 * torch.special.erfc(-wide / 2 ** 0.5), torch.exp(-wide * wide / 2) / (2 * torch.pi) ** 0.5
+    # cdf = 0.5 + z R(z^2): R to 2.5 roundings of its value, the sum rounded once; the product with z once more
+    cdferr = E * (cdf + 2.5 * (cdf - 0.5).abs())
+    within(ctx.linear(z, one, act="gelu"), wide * cdf, wide.abs() * (cdferr + E * cdf) + 1e-44)
+    # z times the density: a product, the exponential's argument (two roundings of at most 1.04) and its own step: 5 in all
+    want = cdf + wide * density
+    dx, _, _ = ctx.linear_backward(torch.ones_like(z), z, one, pre=z, act="gelu")
+    within(dx, want, cdferr + 5 * E * (wide * density).abs() + E * want.abs())
