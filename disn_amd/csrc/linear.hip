@@ -110,6 +110,20 @@ __device__ __forceinline__ float gated(float dy, float z, int act) {
   }
 }
 
+template <typename T, int N, typename Z>
+__device__ __forceinline__ void gate_all(float (&dy)[N], const Z& z, int act) {
+  if (act == DISN_ACT_RELU) {   // one branch for all of them
+#pragma unroll
+    for (int i = 0; i < N; ++i) dy[i] = gated<T>(dy[i], (float)z[i], DISN_ACT_RELU);
+  } else if (act == DISN_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) dy[i] = gated<T>(dy[i], (float)z[i], DISN_ACT_GELU);
+  } else if (act == DISN_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) dy[i] = gated<T>(dy[i], (float)z[i], DISN_ACT_SILU);
+  }
+}
+
 // ---- what becomes of a finished sum ------------------------------------------------------------------------------
 struct Epilogue {
   const void *bias, *residual;
@@ -990,8 +1004,10 @@ __device__ __forceinline__ floatx4 small_operand(const SmallOperand& o, int i, i
   if constexpr (GATED) {
     if (act != DISN_ACT_NONE) {
       const floatx4 z = load_4r<T, ACROSS, FULL>(o.gate, o.ldg, i, r0, K);
+      float g[4] = {v[0], v[1], v[2], v[3]};
+      gate_all<T>(g, z, act);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = FULL || r0 + e < K ? gated<T>(v[e], z[e], act) : 0.0f;
+      for (int e = 0; e < 4; ++e) v[e] = FULL || r0 + e < K ? g[e] : 0.0f;
     }
   }
   return v;
@@ -1368,7 +1384,8 @@ __global__ __launch_bounds__(256) void k_gate(GateArgs a) {
       }
       float v[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = a.act != DISN_ACT_NONE ? gated<T>((float)g[u].v[i], (float)z[u].v[i], a.act) : (float)g[u].v[i];
+      for (int i = 0; i < V; ++i) v[i] = (float)g[u].v[i];
+      if (a.act != DISN_ACT_NONE) gate_all<T>(v, z[u].v, a.act);
       if (a.dz && n > 0) {
         T* dz = (T*)a.dz + row * a.ldz + col;
         if constexpr (SINGLE) {
