@@ -373,9 +373,9 @@ __device__ __forceinline__ floatx16 mfma(shortx8 a, shortx8 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-template <typename T, bool ACROSS, int ROWS, int THREADS, int DEPTH>
+template <bool ACROSS, int ROWS, int THREADS, int DEPTH>
 struct Operand {
-  static constexpr int KT = KT32, P = PLANES, V = Vec<T>::N;
+  static constexpr int KT = KT32, P = PLANES, V = Vec<float>::N;
   static constexpr int PER_LINE = (ACROSS ? ROWS : KT) / V;    // 16-byte pieces in a contiguous run
   static constexpr int Q = ROWS * KT / V / THREADS;            // pieces a thread moves per stage
   static constexpr int LINE = ROWS * 2 + 64;                   // bytes of one r (across)
@@ -384,15 +384,15 @@ struct Operand {
   static constexpr int BYTES = PLANE * P;
   static_assert(Q * THREADS * V == ROWS * KT, "pieces");
 
-  const T* ptr[Q];
+  const float* ptr[Q];
   int64_t ld;
   int left;          // i values in the tile
   int first;         // the stage's first value in its row
   int lines;         // i values in the matrix
   int back[ACROSS ? Q : 1];   // how far in front a piece is read in whole stages (inside() lines)
-  Vec<T> reg[DEPTH][Q];   // stages under way
+  Vec<float> reg[DEPTH][Q];   // stages under way
 
-  __device__ __forceinline__ void init(const T* p, int64_t ld_, int i0, int n_i, int64_t k0) {
+  __device__ __forceinline__ void init(const float* p, int64_t ld_, int i0, int n_i, int64_t k0) {
     ld = ld_;
     left = n_i - i0;
     first = ACROSS ? i0 : (int)k0;
@@ -577,11 +577,11 @@ __device__ __forceinline__ void fp32_sums(const TileArgs& a, int iw, int jw, int
   if (r < have) step(r, std::false_type());
 }
 
-template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int DEPTH>
+template <bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int DEPTH>
 __device__ __forceinline__ void tile32(const TileArgs& a, int block, char* lds) {
   constexpr int THREADS = WM * WN * 64, MB = BM / WM / 32, NB = BN / WN / 32, KT = KT32, P = PLANES;
-  typedef Operand<T, A_ACROSS, BM, THREADS, DEPTH> OpA;
-  typedef Operand<T, B_ACROSS, BN, THREADS, DEPTH> OpB;
+  typedef Operand<A_ACROSS, BM, THREADS, DEPTH> OpA;
+  typedef Operand<B_ACROSS, BN, THREADS, DEPTH> OpB;
   constexpr int BUF = OpA::BYTES + OpB::BYTES;
   const TilePlace at = tile_place(a, block, BM, BN);
   const int i0 = at.i0, j0 = at.j0, split = at.split;
@@ -601,8 +601,8 @@ __device__ __forceinline__ void tile32(const TileArgs& a, int block, char* lds) 
   OpA A;
   OpB B;
   uint32_t lost = 0;
-  A.init((const T*)a.A, a.lda, i0, a.M, k0);
-  B.init((const T*)a.B, a.ldb, j0, a.N, k0);
+  A.init((const float*)a.A, a.lda, i0, a.M, k0);
+  B.init((const float*)a.B, a.ldb, j0, a.N, k0);
   auto multiply = [&](int buffer) {
     const char* cur = lds + buffer * BUF;
 #pragma unroll
@@ -619,12 +619,12 @@ __device__ __forceinline__ void tile32(const TileArgs& a, int block, char* lds) 
         for (int p = 0; p < P; ++p) f[p] = OpA::fragment(cur, p, wi + m * 32, q);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          acc[m][n] = mfma<T>(f[2], b[n][0], acc[m][n]);
-          acc[m][n] = mfma<T>(f[0], b[n][2], acc[m][n]);
-          acc[m][n] = mfma<T>(f[1], b[n][1], acc[m][n]);
-          acc[m][n] = mfma<T>(f[1], b[n][0], acc[m][n]);
-          acc[m][n] = mfma<T>(f[0], b[n][1], acc[m][n]);
-          acc[m][n] = mfma<T>(f[0], b[n][0], acc[m][n]);
+          acc[m][n] = mfma<bf16_t>(f[2], b[n][0], acc[m][n]);
+          acc[m][n] = mfma<bf16_t>(f[0], b[n][2], acc[m][n]);
+          acc[m][n] = mfma<bf16_t>(f[1], b[n][1], acc[m][n]);
+          acc[m][n] = mfma<bf16_t>(f[1], b[n][0], acc[m][n]);
+          acc[m][n] = mfma<bf16_t>(f[0], b[n][1], acc[m][n]);
+          acc[m][n] = mfma<bf16_t>(f[0], b[n][0], acc[m][n]);
         }
       }
     }
@@ -719,13 +719,13 @@ __device__ __forceinline__ void tile32(const TileArgs& a, int block, char* lds) 
     }
     if (again) fp32_sums<A_ACROSS, B_ACROSS, MB, NB>(a, i0 + wi, j0 + wj, k0, have, acc);
   }
-  tile_end<T, MB, NB, WM * WN>(a, split, i0 + wi, j0 + wj, acc, (float*)lds);
+  tile_end<float, MB, NB, WM * WN>(a, split, i0 + wi, j0 + wj, acc, (float*)lds);
 }
 
-template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int DEPTH>
+template <bool A_ACROSS, bool B_ACROSS, int BM, int BN, int WM, int WN, int DEPTH>
 __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile32(TileArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  tile32<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN, DEPTH>(a, blockIdx.x, lds);
+  tile32<A_ACROSS, B_ACROSS, BM, BN, WM, WN, DEPTH>(a, blockIdx.x, lds);
 }
 
 // ---- k_tile16 ------------------------------------------------------------------------------------------------------
@@ -957,8 +957,8 @@ __global__ __launch_bounds__(256, 2) void k_tile_pair(TileArgs dx, TileArgs dw, 
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int block = blockIdx.x;
   if constexpr (sizeof(T) == 4) {
-    if (block < split) tile32<T, false, W_NK, 128, 128, 2, 2, 2>(dx, block, lds);
-    else tile32<T, true, true, 128, 128, 2, 2, 2>(dw, block - split, lds);
+    if (block < split) tile32<false, W_NK, 128, 128, 2, 2, 2>(dx, block, lds);
+    else tile32<true, true, 128, 128, 2, 2, 2>(dw, block - split, lds);
   } else {
     if (block < split) tile16<T, false, W_NK, 128, 128, 2, 2, 4>(dx, block, lds);
     else tile16<T, true, true, 128, 128, 2, 2, 4>(dw, block - split, lds);
@@ -1622,7 +1622,7 @@ int launch_finish(DisnCtx* ctx, const float* part, int nparts, int64_t M, int64_
 template <typename T, bool A_ACROSS, bool B_ACROSS, int BM, int BN, int THREADS, int RING>
 constexpr int tile_lds() {
   if constexpr (sizeof(T) == 4)
-    return 2 * (Operand<T, A_ACROSS, BM, THREADS, 1>::BYTES + Operand<T, B_ACROSS, BN, THREADS, 1>::BYTES);
+    return 2 * (Operand<A_ACROSS, BM, THREADS, 1>::BYTES + Operand<B_ACROSS, BN, THREADS, 1>::BYTES);
   else
     return RING * (BM + BN) * KT16 * 2;
 }
@@ -1644,7 +1644,7 @@ int launch_tile(DisnCtx* ctx, TileArgs a, hipStream_t stream) {
   constexpr int THREADS = WM * WN * 64;
   const void* kernel;
   if constexpr (sizeof(T) == 4)   // (a stage of a 128-wide tile is over before the next has come: two under way)
-    kernel = (const void*)k_tile32<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN, BM == 128 ? 2 : 1>;
+    kernel = (const void*)k_tile32<A_ACROSS, B_ACROSS, BM, BN, WM, WN, BM == 128 ? 2 : 1>;
   else
     kernel = (const void*)k_tile16<T, A_ACROSS, B_ACROSS, BM, BN, WM, WN, RING>;
   static std::atomic<uint64_t> ready{0};
@@ -1710,7 +1710,7 @@ void launch_thin(const Product& q, const Plan& p, float* part, hipStream_t strea
   else k_thin<THIN><<<blocks, 256, 0, stream>>>(a);
 }
 
-SmallArgs small_args(const Product& q, const Plan&) {
+SmallArgs small_args(const Product& q) {
   SmallArgs s{};
   s.A = {q.A, nullptr, q.lda, 0}, s.B = {q.B, nullptr, q.ldb, 0};
   s.M = (int)q.M, s.N = (int)q.N, s.K = (int)q.K;
@@ -1746,7 +1746,7 @@ int run_product(DisnCtx* ctx, Product q, Plan p, char* ws, hipStream_t stream) {
   if (q.M == 0 || q.N == 0) return DISN_OK;
   if (p.kind == K_EMPTY) return launch_finish<T>(ctx, nullptr, 0, q.M, q.N, q.e, stream);
   if (p.kind == K_SMALL) {
-    const SmallArgs s = small_args(q, p);
+    const SmallArgs s = small_args(q);
     const unsigned blocks = (unsigned)small_blocks(s);
     if (q.a_across) {
       // dW beside a large dx: the paired kernel without a dx
@@ -1941,7 +1941,7 @@ int run_backward(DisnCtx* ctx, const DisnLinearGrad* a, const GradPlan& g, char*
     if (a->dw) DISN_TRY(run_product<T>(ctx, dw, g.dw, ws + g.off_part, stream));
     return DISN_OK;
   }
-  SmallArgs sx = small_args(dx, g.dx), sw = small_args(dw, g.dw);
+  SmallArgs sx = small_args(dx), sw = small_args(dw);
   sx.act = sw.act = a->act;
   sx.A.gate = a->pre, sx.A.ldg = a->ldp;
   SmallOperand& of = a->w_nk ? sw.A : sw.B;
