@@ -349,7 +349,8 @@ class Context:
         """Gradients of linear (disn_linear_backward) -> (dx, dw, db), None for the ones not wanted.  dy: [..., n];
         x, w as in linear (w may be None without dx, x without dw); pre: linear's second result, not with act
         "none"; for relu without a residual y does as well.  dw lies in memory as w does.  The gradient of the
-        residual is dy."""
+        residual is dy.  A closed relu passes 0 whatever dy holds.  In 16 bits the gradient behind an activation is rounded to the
+        type before the two products, unless the call is small."""
         if self._elsewhere():
             with torch.cuda.device(self.device):
                 return self.linear_backward(dy, x, w, pre, act, want_dx, want_dw, want_db)

@@ -186,13 +186,14 @@ int disn_vgg_forward(DisnCtx* ctx, int slot, const float* img, int img_h, int im
  *    ld = 0: one row for all).  Any base address that fits the type is allowed.  Up to 2^30 rows (m, rows); n and k of
  *    a dense layer up to DISN_LINEAR_MAX
  *  - a size of zero is fine: an empty output is not written, a sum over nothing is 0
- *  - an output must not overlap any other argument.  One exception: y of disn_linear may be the residual itself
- *    (same address and ld)
+ *  - an output must not overlap any other argument; the caller sees to it, the calls do not look.  One exception: y of
+ *    disn_linear may be the residual itself (same address and ld)
  *  - the workspace (DEVICE, 16-byte aligned, any contents, free again when the stream has passed the call) belongs to
  *    the caller: its size comes from the *_workspace call on the same arguments (0: may be NULL).  The calls allocate
  *    nothing, keep nothing and clear nothing through the runtime, so they can be captured into graphs; two graphs or
  *    streams that may run at the same time need a workspace each
- *  - results do not depend on the run: fixed summation orders, no atomics */
+ *  - results do not depend on the run: fixed summation orders, no atomics; nor on what lies beside a matrix or in the
+ *    workspace */
 #define DISN_F32 0
 #define DISN_BF16 1
 #define DISN_F16 2
@@ -229,8 +230,10 @@ int disn_linear(DisnCtx* ctx, const DisnLinear* a, void* workspace, size_t works
  *   dy [m][n] (also the gradient of the residual);  pre [m][n]: z as disn_linear returned it, NULL with
  *   DISN_ACT_NONE; for DISN_ACT_RELU any tensor that is positive where z is does, y of a call without residual too
  *   dx [m][k], dw (layout w_nk, like w), db [n]: NULL = not wanted; w may be NULL without dx, x without dw
- * Where pre is NaN, dz is NaN.  16-bit types: dz is rounded to the type before the two products (they take 16-bit
- * operands) unless act is none. */
+ * Where pre is NaN, dz is NaN.  16-bit types with an activation: the two products take dz rounded to the type (the matrix
+ * instructions' operands), so a |dz| beyond the type's largest value (fp16: 65504) is infinite there and one below half
+ * of its smallest (2^-25) 0; db is summed from dz in fp32.  Calls that are small enough for one launch (chosen by m, n and k)
+ * keep dz in fp32 for the products too: scale losses as for any fp16 tensor. */
 typedef struct DisnLinearGrad {
   int32_t type, act, w_nk, reserved; /* reserved = 0 */
   int64_t m, n, k;
