@@ -350,10 +350,10 @@ __device__ __forceinline__ TilePlace tile_place(const TileArgs& a, int block, in
 // A workgroup computes a BM x BN tile of C, r in stages of KT.  The stage after the next is on its way from memory to
 // registers while the next lies in one LDS buffer and the waves multiply the present one from the other: one barrier a
 // stage.  Waves are WM x WN; each has MB x NB tiles of v_mfma_f32_32x32x16.  Bound by the matrix cores: 100000 x 1984 x 512
-// 980 us, 4096^3 605 us (227 TFLOP/s; an fp32 library product on the fp32 matrix instructions 138).
+// 940 us, 4096^3 605 us (227 TFLOP/s; an fp32 library product on the fp32 matrix instructions 138).
 //
-// For fp32, which is cut into three bf16 terms x = h + m + l (each the rounded
-// rest of the one before; 8 + 8 + 8 bits hold fp32's 24, so the sum is exact) and the six products
+// An fp32 value is cut into three bf16 terms x = h + m + l (each the rounded
+// rest of the one before; 8 + 8 + 8 bits hold fp32's 24, so the sum is exact), and the six products
 // hh, hm, mh, mm, hl, lh are accumulated in fp32; what is left out (ml, lm, ll) is below 2^-24 of a product, as an
 // FMA's rounding is.  Six bf16 MFMAs take 6/16 of the time of one fp32 MFMA of the same size.  Infinities,
 // NaN and intermediate overflow cannot be cut; a tile whose sums are not all finite is computed again by fp32 MFMAs.
@@ -734,7 +734,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile32(TileArgs a) {
 // the fragments of a step are read while the step before is multiplied; the one barrier of a stage lies between its two
 // steps, when the second step's fragments are in registers: no wave waits for LDS behind it.  Bound by the matrix cores, then
 // by the epilogue, which no other workgroup of the CU covers: 65536 x 1536 x 512 bf16 91 us (1.13 PFLOP/s), its weight's
-// gradient 88 and the input's, with three times the results, 117; 4096^3 113 to 125 (a library product 104 to 125).
+// gradient 86 and the input's, with three times the results, 117; 4096^3 110 to 125 (a library product 91 to 125).
 //
 // A wave's DMA writes 1 KB of LDS in lane order, from any 16-byte pieces of memory.  Along r, LDS holds [i][32 r] (64
 // bytes), and the four pieces of a row are exchanged by (i >> 2) & 3: sixteen lanes of a fragment, sixteen rows, touch
@@ -1339,7 +1339,7 @@ __global__ __launch_bounds__(256) void k_thin(ThinArgs a) {
 
 // ---- dz = dy act'(pre) and partial column sums of it -------------------------------------------------------------------
 // A lane owns 16 bytes of columns (SINGLE: one, for rows of less than 16 bytes); rows narrower than a wave put several of them
-// into it.  Four rows are under way.  Bound by memory: 65536 x 512 bf16 relu 41 us, 4.9 TB/s
+// into it.  Four rows are under way.  Bound by memory: 65536 x 512 bf16 relu 38 us, 5.3 TB/s
 // of the three matrices.
 struct GateArgs {
   const void *dy, *pre;
@@ -1447,8 +1447,10 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 //   16 bits    9.5, 17                 9.5, 25                 5.5, 7.5     7, 16.5     7.7, 25.5
 //   fp32       14, 105                 14, 145                 9.2, 50      9, 85
 // Split sums are written and read once more in fp32, at 10 TB/s while they fit the last cache, by one more launch (4 us).
-// Measured (estimated): gradient of a 1536 x 512 weight over 65536 bf16 rows 256-wide / 21 parts 103 (105), 128-wide / 10 parts
-// 127 (125); 4096 x 4096, r = 2048 256-wide 61 (61), 128-wide 86 (81); 2048 x 2048, r = 2048, 256-wide / 4 parts 39 (40).
+// Measured (estimated): gradient of a 1536 x 512 weight over 65536 bf16 rows 256-wide / 21 parts 107 (105), 128-wide / 10 parts
+// 136 (125); 4096 x 4096, r = 2048 256-wide 59 (61), 128-wide 89 (81); 2048 x 2048, r = 2048, 256-wide / 4 parts 39 (40), 128-wide
+// 23.  The table's kernels, measured again with results stored past the caches, lie within 10 % of it.  What a tile's end does is not
+// priced: 10007 x 777 fp16 results of r = 1000 with a gelu, a residual and z are estimated at 28 and take 50.
 // A last round that is at most half full is not started (operands that are copied first aside): the rows before it are one
 // launch, the others another (100000 x 512 fp32 outputs are 782 tiles, three rounds and 14 tiles).
 struct TileChoice {
