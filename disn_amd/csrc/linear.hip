@@ -62,7 +62,19 @@ __device__ __forceinline__ float normal_cdf(float z, float& e) {
   r = fmaf(r, s, 0.3989423f);
   return s < 1.5f ? fmaf(z, r, 0.5f) : p;
 }
-__device__ __forceinline__ float logistic(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
+// 1 / (1 + exp(-z)).  The product with log2 e is rounded, which is |z| 2^-24 of the exponential: nothing beside half a step of a 16-bit
+// result, but 1e-6 of silu at -10 in float32, where what the product and its constant lost is made up for (not where the
+// exponential is infinite or 0).
+template <typename T>
+__device__ __forceinline__ float logistic(float z) {
+  const float t = z * -1.44269504f;
+  float p = __builtin_amdgcn_exp2f(t);
+  if constexpr (sizeof(T) == 4) {
+    const float lost = fmaf(z, -1.92596299e-8f, fmaf(z, -1.44269504f, -t));
+    p = fabsf(z) < 88.0f ? fmaf(p, lost * 0.69314718f, p) : p;
+  }
+  return __builtin_amdgcn_rcpf(1.0f + p);
+}
 
 // T: the type of the result
 template <typename T>
@@ -71,7 +83,7 @@ __device__ __forceinline__ float activate(float z, int act) {
   switch (act) {
     case DISN_ACT_RELU: return z < 0.0f ? 0.0f : z;   // NaN stays
     case DISN_ACT_GELU: return z * normal_cdf<T>(z, e);
-    case DISN_ACT_SILU: return z * logistic(z);
+    case DISN_ACT_SILU: return z * logistic<T>(z);
     default: return z;
   }
 }
@@ -103,7 +115,7 @@ __device__ __forceinline__ float gated(float dy, float z, int act) {
       return dy * fmaf(z * 0.39894228f, e, p);
     }
     case DISN_ACT_SILU: {
-      const float s = logistic(z);
+      const float s = logistic<T>(z);
       return dy * (s * fmaf(z, 1.0f - s, 1.0f));
     }
     default: return dy;

@@ -180,3 +180,21 @@ def test_gelu_of_float32(ctx):
     want = cdf + wide * density
     dx, _, _ = ctx.linear_backward(torch.ones_like(z), z, one, pre=z, act="gelu")
     within(dx, want, cdferr + 5 * E * (wide * density).abs() + E * want.abs())
+
+
+def test_silu_of_float32(ctx):
+    """silu and its slope over the whole range of their exponential, to the roundings of a few operations"""
+    g = gen("silu")
+    z = torch.cat([torch.rand(60000, 1, generator=g, device=DEV) * 110 - 80, torch.randn(20000, 1, generator=g, device=DEV)])
+    one = torch.ones(1, 1, device=DEV)
+    wide = z.double()
+    s = torch.sigmoid(wide)
+    # the exponential and the reciprocal to a step (2 E) each, three roundings of s, one of the product
+    within(ctx.linear(z, one, act="silu"), wide * s, 8 * E * (wide * s).abs() + 1e-36)
+    # s (1 + z (1 - s)): s to 7 E, 1 - s to 7 E s + E, two roundings of the sum, one of the product
+    want = s * (1 + wide * (1 - s))
+    dx, _, _ = ctx.linear_backward(torch.ones_like(z), z, one, pre=z, act="silu")
+    within(dx, want, E * (8 * want.abs() + s * (2 + wide.abs() * (7 * s + 3 * (1 - s)))) + 1e-36)
+    big = torch.tensor([[-1e30], [-200.0], [-100.0], [100.0], [1e30], [float("inf")], [float("nan")]], device=DEV)
+    y = ctx.linear(big, one, act="silu")[:, 0]
+    assert (y[:3].abs() <= 1e-36).all() and torch.equal(y[3:6], big[3:6, 0]) and y[6].isnan()
